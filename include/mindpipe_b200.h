@@ -744,6 +744,67 @@ int mp_moe_combine_after_peers(const void* arrival_words_u32, int world, const v
 int mp_gather_rows(const void* src, const void* row_map_i32, int n_dst_rows, int row_bytes, void* dst,
                    mp_stream_t stream);
 
+/* -------------------------------------------------------------- attention */
+
+/*
+ * Between qkv_proj and o_proj of a decoder layer: a paged cache of keys and values, what fills it, what reads it, and
+ * attention of whole prompts -- the place of the runtime's attention path
+ * (npu_fused_infer_attention_score, acceleration/runtime_patches/vllm_ascend.patch:141-291).
+ *
+ * dtype: 0 = f16, 1 = bf16, the same for all operands of a call.  D % 8 == 0, 8 <= D <= 128.  Data pointers and strides
+ * are multiples of 16 bytes; strides count values and may not be negative; the last dimension is dense.
+ * index_word (device int, may be null): set to 1 where a position, slot, page, length or sequence end that a kernel reads is
+ * out of range.  Nothing outside the operands is touched then, and the results of the rows concerned are unspecified.
+ */
+typedef struct {
+  const void* data;            /* [rows, heads, D] */
+  long long token_stride;
+  long long head_stride;
+} mp_head_rows;
+
+typedef struct {
+  void* k;                     /* [pages, kv_heads, page_size, D] each, with strides of their own */
+  void* v;
+  int pages, kv_heads, page_size;
+  long long k_page_stride, k_head_stride, k_token_stride;
+  long long v_page_stride, v_head_stride, v_token_stride;
+} mp_paged_cache;
+
+/*
+ * Rotates the first `rotated` values of every head of q[T,Hq,D] and k[T,Hkv,D] by the angles of the tokens' positions and
+ * stores keys and values v[T,Hkv,D] in the cache: token t goes to offset slots[t] % page_size of page slots[t] / page_size,
+ * or nowhere where slots[t] < 0.  cos_sin f32 [max_positions, rotated]: a row holds the cosines of the rotated / 2 angles,
+ * then their sines.  Pairs are (i, i + rotated / 2), or (2i, 2i + 1) with interleaved != 0; arithmetic in fp32, one
+ * rounding.  q_out [T,Hq,D] and, unless null, k_out [T,Hkv,D] get the rotated queries and keys.  2 <= rotated <= D, even.
+ * A token with a negative slot may have any position; one out of range then counts as 0.  Slots that occur twice
+ * in a call are left with values of either token.  q_out and k_out may not overlap the inputs.
+ */
+int mp_rotary_append_paged(int dtype, const mp_head_rows* q, const mp_head_rows* k, const mp_head_rows* v,
+                           const void* cos_sin_f32, int max_positions, int rotated, int interleaved,
+                           const void* positions_i32, const void* slots_i32, int T, int Hq, int D,
+                           const mp_paged_cache* cache, void* q_out, void* k_out, int* index_word, mp_stream_t stream);
+
+/*
+ * out[B,Hq,D] = softmax(scale q K^T) V over the first seq_lens[b] tokens in the pages page_table[b, :] names
+ * (int32 [B, table_pages], entries behind the last token's page are not read); seq_lens[b] == 0 gives zeros.  Query head i
+ * attends to the keys of head i / (Hq / kv_heads).  The cache is read once, split evenly over the SMs whatever the
+ * lengths; parts of a sequence are joined through the workspace (zero-filled once when it is created, left so by every
+ * call, not shared by calls that may overlap).
+ */
+size_t mp_paged_attention_decode_workspace_bytes(void);
+int mp_paged_attention_decode(int dtype, const mp_head_rows* q, int B, int Hq, int D, const mp_paged_cache* cache,
+                              const void* page_table_i32, int table_pages, const void* seq_lens_i32, float scale, void* out,
+                              void* workspace, size_t workspace_bytes, int* index_word, mp_stream_t stream);
+
+/*
+ * Causal attention within packed sequences: rows cu_seqlens[b] .. cu_seqlens[b+1] of q[T,Hq,D], k and v[T,Hkv,D] are
+ * sequence b (int32 [B + 1], ascending, at most T), and its row i attends to its rows 0..i.  Rows of out[T,Hq,D] that
+ * belong to no sequence are left as they are.
+ */
+int mp_attention_prefill(int dtype, const mp_head_rows* q, const mp_head_rows* k, const mp_head_rows* v, int T, int Hq,
+                         int Hkv, int D, const void* cu_seqlens_i32, int B, float scale, void* out, int* index_word,
+                         int* error_word, mp_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

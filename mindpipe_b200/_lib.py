@@ -101,6 +101,10 @@ SIGNATURES = {
     "mp_moe_ep_push_part": (_I, [_P, _P, _I, _I, _I, _I, _P, _I, _P]),
     "mp_moe_ep_push_signal": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _I, _P, _P, _P]),
     "mp_moe_combine_after_peers": (_I, [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P]),
+    "mp_rotary_append_paged": (_I, [_I, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P]),
+    "mp_paged_attention_decode_workspace_bytes": (_Z, []),
+    "mp_paged_attention_decode": (_I, [_I, _P, _I, _I, _I, _P, _P, _I, _P, ctypes.c_float, _P, _P, _Z, _P, _P]),
+    "mp_attention_prefill": (_I, [_I, _P, _P, _P, _I, _I, _I, _I, _P, _I, ctypes.c_float, _P, _P, _P, _P]),
 }
 
 
@@ -110,6 +114,17 @@ class HostLinear(ctypes.Structure):
                 ("bias_f16", c_void_p), ("y_stage_f16", c_void_p), ("y_host_f16", c_void_p),
                 ("M", c_int), ("N", c_int), ("K", c_int), ("group", c_int),
                 ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class HeadRows(ctypes.Structure):
+    """``mp_head_rows`` of the C header."""
+    _fields_ = [("data", c_void_p), ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
+
+
+class PagedCache(ctypes.Structure):
+    """``mp_paged_cache`` of the C header."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("pages", c_int), ("kv_heads", c_int), ("page_size", c_int)] + \
+        [(f"{side}_{name}_stride", ctypes.c_longlong) for side in "kv" for name in ("page", "head", "token")]
 
 
 class MindPipeKernelError(RuntimeError):

@@ -22,6 +22,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -39,8 +40,8 @@ namespace {
 // decode kernels leave their part zeroed where it has to be, so it is cleared only when it is (re)allocated; the kinds whose
 // kernels overwrite theirs freely (split-K partial sums) have buffers of their own.  Launches of one stream run in order, so
 // they may share.
-enum WorkspaceKind { kDecode = 0, kPrefill = 1, kW8A8 = 2, kKinds = 3 };
-const char* const kKindNames[kKinds] = {"decode", "prefill", "w8a8"};
+enum WorkspaceKind { kDecode = 0, kPrefill = 1, kW8A8 = 2, kAttention = 3, kKinds = 4 };
+const char* const kKindNames[kKinds] = {"decode", "prefill", "w8a8", "attention"};
 
 std::mutex g_workspace_mutex;
 std::map<std::tuple<int, cudaStream_t, int>, at::Tensor> g_workspaces;
@@ -544,6 +545,217 @@ PyObject* w4_dequant(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
+// --------------------------------------------------------------------------------------------------------- attention
+// The wrappers' checks in native code: a decode step's launches take 3-5 us each, the same checks in Python twice that.
+// A false or null return has a Python error set.
+struct AttentionCall {
+  at::ScalarType dtype = at::kHalf;
+  int device = -1;
+
+  bool tensor(PyObject* o, const char* name, const at::Tensor** out, int ndim) {
+    if (!THPVariable_Check(o)) {
+      PyErr_Format(PyExc_TypeError, "%s must be a tensor", name);
+      return false;
+    }
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda()) {
+      PyErr_Format(PyExc_ValueError, "%s must be a CUDA tensor (there is no CPU path)", name);
+      return false;
+    }
+    if (t.dim() != ndim) {
+      PyErr_Format(PyExc_ValueError, "%s must be %dD, got %dD", name, ndim, static_cast<int>(t.dim()));
+      return false;
+    }
+    if (device < 0) device = t.get_device();
+    if (t.get_device() != device) {
+      PyErr_Format(PyExc_ValueError, "%s is on another device than the other operands", name);
+      return false;
+    }
+    for (int64_t n : t.sizes())
+      if (n > 0x7fffffff) {
+        PyErr_Format(PyExc_ValueError, "%s has a dimension above 2^31 - 1", name);
+        return false;
+      }
+    *out = &t;
+    return true;
+  }
+  // dense operands of a fixed type
+  bool dense(PyObject* o, const char* name, const at::Tensor** out, int ndim, at::ScalarType want) {
+    if (!tensor(o, name, out, ndim)) return false;
+    if ((*out)->scalar_type() != want) {
+      PyErr_Format(PyExc_TypeError, "%s must be %s, got %s", name, c10::toString(want), c10::toString((*out)->scalar_type()));
+      return false;
+    }
+    if (!(*out)->is_contiguous()) {
+      PyErr_Format(PyExc_ValueError, "%s must be contiguous", name);
+      return false;
+    }
+    return true;
+  }
+  // the 16-bit operands: the first one decides the type, all have a dense last dimension and the rest in steps of 16 bytes
+  bool values(PyObject* o, const char* name, const at::Tensor** out, int ndim, bool first = false) {
+    if (!tensor(o, name, out, ndim)) return false;
+    const at::Tensor& t = **out;
+    if (first) dtype = t.scalar_type();
+    if ((dtype != at::kHalf && dtype != at::kBFloat16) || t.scalar_type() != dtype) {
+      PyErr_Format(PyExc_TypeError, "%s must be float16 or bfloat16, as the other operands, got %s", name,
+                   c10::toString(t.scalar_type()));
+      return false;
+    }
+    const int64_t d = t.size(ndim - 1);
+    if (d % 8 || d < 8 || d > 128) {
+      PyErr_Format(PyExc_ValueError, "%s: heads of 8 to 128 values, a multiple of 8; got %lld", name, static_cast<long long>(d));
+      return false;
+    }
+    bool ok = t.stride(ndim - 1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int i = 0; i + 1 < ndim; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+    if (!ok) {
+      PyErr_Format(PyExc_ValueError, "%s: the last dimension must be dense, the others begin at multiples of 16 bytes", name);
+      return false;
+    }
+    return true;
+  }
+  bool fail(const char* what) {
+    PyErr_SetString(PyExc_ValueError, what);
+    return false;
+  }
+  int type() const { return dtype == at::kHalf ? 0 : 1; }
+};
+
+// a dimension of one entry may have any stride
+long long stride_of(const at::Tensor& t, int i) { return t.size(i) <= 1 ? 0 : t.stride(i); }
+
+mp_head_rows head_rows(const at::Tensor& t) { return mp_head_rows{t.data_ptr(), stride_of(t, 0), stride_of(t, 1)}; }
+
+// the cache as k_cache and v_cache [pages, kv heads, page size, D]
+bool cache_arg(AttentionCall& call, PyObject* ko, PyObject* vo, const at::Tensor** k, mp_paged_cache* c) {
+  const at::Tensor* v;
+  if (!call.values(ko, "k_cache", k, 4) || !call.values(vo, "v_cache", &v, 4)) return false;
+  if ((*k)->sizes() != v->sizes()) return call.fail("k_cache and v_cache shapes differ");
+  if ((*k)->numel() == 0) return call.fail("the cache is empty");
+  *c = mp_paged_cache{(*k)->data_ptr(), v->data_ptr(), static_cast<int>((*k)->size(0)), static_cast<int>((*k)->size(1)),
+                      static_cast<int>((*k)->size(2)), stride_of(**k, 0), stride_of(**k, 1), stride_of(**k, 2),
+                      stride_of(*v, 0), stride_of(*v, 1), stride_of(*v, 2)};
+  return true;
+}
+
+at::Tensor dense_like(const at::Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
+
+// an output the caller brought, or a new one; null with an error set
+bool output_arg(AttentionCall& call, PyObject* o, const at::Tensor& like, at::Tensor* out) {
+  if (o == Py_None) {
+    *out = dense_like(like);
+    return true;
+  }
+  const at::Tensor* t;
+  if (!call.values(o, "out", &t, 3)) return false;
+  if (t->sizes() != like.sizes() || !t->is_contiguous()) return call.fail("out must be contiguous and shaped like q");
+  *out = *t;
+  return true;
+}
+
+// (q_out, k_out or None), or the error status as an int
+PyObject* rotary_append(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *qo, *ko, *vo, *to, *po, *so, *kco, *vco;
+  int interleaved, want_k;
+  unsigned long long word;
+  if (!PyArg_ParseTuple(args, "OOOOOOOOppK", &qo, &ko, &vo, &to, &po, &so, &kco, &vco, &interleaved, &want_k, &word)) return nullptr;
+  AttentionCall call;
+  const at::Tensor *q, *k, *v, *table, *pos, *slots, *kc;
+  mp_paged_cache cache;
+  if (!call.values(qo, "q", &q, 3, true) || !call.values(ko, "k", &k, 3) || !call.values(vo, "v", &v, 3) ||
+      !call.dense(to, "cos_sin", &table, 2, at::kFloat) || !call.dense(po, "positions", &pos, 1, at::kInt) ||
+      !call.dense(so, "slots", &slots, 1, at::kInt) || !cache_arg(call, kco, vco, &kc, &cache))
+    return nullptr;
+  const int64_t t = q->size(0), d = q->size(2), rotated = table->size(1);
+  if (k->sizes() != v->sizes() || k->size(0) != t || k->size(2) != d || k->size(1) != cache.kv_heads || kc->size(3) != d)
+    return call.fail("q, k, v and cache shapes are inconsistent"), nullptr;
+  if (pos->size(0) != t || slots->size(0) != t) return call.fail("positions and slots must have one entry per token"), nullptr;
+  if (rotated < 2 || rotated % 2 || rotated > d || table->size(0) == 0 || reinterpret_cast<uintptr_t>(table->data_ptr()) % 16)
+    return call.fail("cos_sin must be [positions, rotated], 16-byte aligned, with an even number of rotated values up to D"), nullptr;
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(call.device));
+  at::Tensor q_out = dense_like(*q), k_out;
+  if (want_k) k_out = dense_like(*k);
+  int rc = MP_OK;
+  if (t && q->size(1)) {
+    const mp_head_rows qr = head_rows(*q), kr = head_rows(*k), vr = head_rows(*v);
+    rc = mp_rotary_append_paged(call.type(), &qr, &kr, &vr, table->data_ptr(), static_cast<int>(table->size(0)),
+                                static_cast<int>(rotated), interleaved, pos->data_ptr(), slots->data_ptr(), static_cast<int>(t),
+                                static_cast<int>(q->size(1)), static_cast<int>(d), &cache, q_out.data_ptr(),
+                                want_k ? k_out.data_ptr() : nullptr, int_pointer(word),
+                                c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(call.device)).stream());
+  }
+  if (rc != MP_OK) return PyLong_FromLong(rc);
+  PyObject* second = want_k ? THPVariable_Wrap(std::move(k_out)) : none();
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(q_out)), second);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* paged_decode(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *qo, *kco, *vco, *to, *lo, *oo, *scale_o;
+  unsigned long long word;
+  if (!PyArg_ParseTuple(args, "OOOOOOOK", &qo, &kco, &vco, &to, &lo, &scale_o, &oo, &word)) return nullptr;
+  AttentionCall call;
+  const at::Tensor *q, *kc, *table, *lens;
+  mp_paged_cache cache;
+  if (!call.values(qo, "q", &q, 3, true) || !cache_arg(call, kco, vco, &kc, &cache) ||
+      !call.dense(to, "page_table", &table, 2, at::kInt) || !call.dense(lo, "seq_lens", &lens, 1, at::kInt))
+    return nullptr;
+  const int64_t b = q->size(0), h = q->size(1), d = q->size(2);
+  if (kc->size(3) != d || h % cache.kv_heads) return call.fail("q and cache shapes are inconsistent"), nullptr;
+  if (table->size(0) != b || lens->size(0) != b || table->size(1) == 0)
+    return call.fail("page_table must be [batch, pages] and seq_lens [batch]"), nullptr;
+  const double scale = scale_o == Py_None ? 1.0 / std::sqrt(static_cast<double>(d)) : PyFloat_AsDouble(scale_o);
+  if (PyErr_Occurred()) return nullptr;
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(call.device));
+  at::Tensor out;
+  if (!output_arg(call, oo, *q, &out)) return nullptr;
+  if (b && h) {
+    const cudaStream_t st = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(call.device)).stream();
+    const Scratch ws(mp_paged_attention_decode_workspace_bytes(), call.device, st, kAttention, true);
+    const mp_head_rows qr = head_rows(*q);
+    const int rc = mp_paged_attention_decode(call.type(), &qr, static_cast<int>(b), static_cast<int>(h), static_cast<int>(d), &cache,
+                                             table->data_ptr(), static_cast<int>(table->size(1)), lens->data_ptr(),
+                                             static_cast<float>(scale), out.data_ptr(), ws.ptr, ws.bytes, int_pointer(word), st);
+    if (rc != MP_OK) return PyLong_FromLong(rc);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* attention_prefill(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *qo, *ko, *vo, *co, *oo, *scale_o;
+  unsigned long long word, error;
+  if (!PyArg_ParseTuple(args, "OOOOOOKK", &qo, &ko, &vo, &co, &scale_o, &oo, &word, &error)) return nullptr;
+  AttentionCall call;
+  const at::Tensor *q, *k, *v, *cu;
+  if (!call.values(qo, "q", &q, 3, true) || !call.values(ko, "k", &k, 3) || !call.values(vo, "v", &v, 3) ||
+      !call.dense(co, "cu_seqlens", &cu, 1, at::kInt))
+    return nullptr;
+  const int64_t t = q->size(0), h = q->size(1), hk = k->size(1), d = q->size(2);
+  if (k->sizes() != v->sizes() || k->size(0) != t || k->size(2) != d || hk == 0 || h % hk)
+    return call.fail("q, k and v shapes are inconsistent"), nullptr;
+  if (cu->size(0) < 1) return call.fail("cu_seqlens must have batch + 1 entries"), nullptr;
+  const double scale = scale_o == Py_None ? 1.0 / std::sqrt(static_cast<double>(d)) : PyFloat_AsDouble(scale_o);
+  if (PyErr_Occurred()) return nullptr;
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(call.device));
+  at::Tensor out;
+  if (!output_arg(call, oo, *q, &out)) return nullptr;
+  if (t && h && cu->size(0) > 1) {
+    const mp_head_rows qr = head_rows(*q), kr = head_rows(*k), vr = head_rows(*v);
+    const int rc = mp_attention_prefill(call.type(), &qr, &kr, &vr, static_cast<int>(t), static_cast<int>(h), static_cast<int>(hk),
+                                        static_cast<int>(d), cu->data_ptr(), static_cast<int>(cu->size(0) - 1),
+                                        static_cast<float>(scale), out.data_ptr(), int_pointer(word), int_pointer(error),
+                                        c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(call.device)).stream());
+    if (rc != MP_OK) return PyLong_FromLong(rc);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_workspace(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
   unsigned long long nbytes;
@@ -592,6 +804,9 @@ PyMethodDef module_methods[] = {{"w4_plan", w4_plan, METH_VARARGS, nullptr},
                                 {"moe_plan", moe_plan, METH_VARARGS, nullptr},
                                 {"w4_quantize", w4_quantize, METH_VARARGS, nullptr},
                                 {"w4_dequant", w4_dequant, METH_VARARGS, nullptr},
+                                {"rotary_append", rotary_append, METH_VARARGS, nullptr},
+                                {"paged_decode", paged_decode, METH_VARARGS, nullptr},
+                                {"attention_prefill", attention_prefill, METH_VARARGS, nullptr},
                                 {"workspace", py_workspace, METH_VARARGS, nullptr},
                                 {"workspaces", py_workspaces, METH_NOARGS, nullptr},
                                 {nullptr, nullptr, 0, nullptr}};

@@ -14,6 +14,7 @@ import torch
 from . import _lib
 
 _err_words: dict[int, torch.Tensor] = {}
+_index_words: dict[int, torch.Tensor] = {}
 
 
 def _stream() -> int:
@@ -351,8 +352,21 @@ def _error_word(device: torch.device) -> torch.Tensor:
     return w
 
 
+def _index_word(device: torch.device) -> int:
+    """Address of the per-device int32 the attention kernels set when an index they read is out of range."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    w = _index_words.get(idx)
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("first use of an attention op must happen outside CUDA graph capture")
+        w = torch.zeros(1, dtype=torch.int32, device=device)
+        _index_words[idx] = w
+    return w.data_ptr()
+
+
 def check_device_errors(device=None) -> None:
-    """Synchronise and raise if any kernel reported a device-side wait that gave up.
+    """Synchronise and raise if any kernel reported a device-side wait that gave up, or an attention kernel an index
+    (position, slot, page, length, sequence end) that was out of range.
 
     A kernel that gave up leaves its arrival counters and partial sums as they were at that moment, so the
     scratch buffers this module caches are cleared again before the error is raised and later calls start from
@@ -378,6 +392,11 @@ def check_device_errors(device=None) -> None:
             w.zero_()
             rearm(idx)
             raise _lib.MindPipeKernelError(f"device {idx}: a bounded wait inside a tensor-core kernel timed out")
+    for idx, w in _index_words.items():
+        if int(w.item()) != 0:
+            w.zero_()
+            raise _lib.MindPipeKernelError(f"device {idx}: an attention call was given a position, slot, page, length or "
+                                           "sequence end out of range")
 
 
 def w8a8_gemm(qx, x_scale, weight_i8, weight_scale, bias=None, *, workspace=None):
@@ -682,4 +701,66 @@ def w8a8_affine_gemm(qx, x_scale, x_zero, x_rowsum, weight_u8, weight_scale, wei
                                          b.data_ptr(), args[3].data_ptr(), args[4].data_ptr(), args[5].data_ptr(),
                                          _ptr(bi), y.data_ptr(), m, n, k, _error_word(a.device).data_ptr(), _stream())
     _lib.check(st, "w8a8_affine_gemm", M=m, N=n, K=k)
+    return y
+
+
+# -------------------------------------------------------------- attention
+def _on_gpu(t, name):
+    """The checks that need no library, so that a machine without a GPU gives the same errors."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    return t.device
+
+
+def rotary_append_paged(q, k, v, cos_sin, positions, slots, k_cache, v_cache, *, interleaved: bool = False,
+                        want_k: bool = False):
+    """Rotate queries and keys by their positions and append keys and values to a paged cache, in one launch.
+
+    ``q [T,Hq,D]``, ``k`` and ``v [T,Hkv,D]`` fp16 or bf16, strided views (of one concatenated projection) included.
+    ``cos_sin`` fp32 ``[positions, rotated]``: a row holds the cosines of a position's ``rotated / 2`` angles, then their
+    sines; the first ``rotated`` values of a head turn, in pairs ``(i, i + rotated / 2)`` or, with ``interleaved``,
+    ``(2i, 2i + 1)``.  Token ``t`` goes to offset ``slots[t] % page_size`` of page ``slots[t] // page_size`` of
+    ``k_cache`` / ``v_cache [pages, Hkv, page_size, D]`` (views with other strides included), or nowhere where
+    ``slots[t] < 0`` (padding); a slot may occur once per call.  ``positions`` and ``slots`` are int32 ``[T]``.
+
+    Returns ``(q_rotated, k_rotated | None)``; the caches are updated in place.  Positions and slots out of range touch no
+    memory and raise at the next :func:`check_device_errors`.
+    """
+    word = _index_word(_on_gpu(q, "q"))
+    made = _lib.host().rotary_append(q, k, v, cos_sin, positions, slots, k_cache, v_cache, interleaved, want_k, word)
+    if isinstance(made, int):
+        _lib.check(made, "rotary_append_paged", q=tuple(q.shape), cache=tuple(k_cache.shape))
+    return made
+
+
+def paged_attention_decode(q, k_cache, v_cache, page_table, seq_lens, *, scale: float | None = None, out=None):
+    """Attention of one new token per sequence over the pages its row of ``page_table`` names.
+
+    ``q [B,Hq,D]`` fp16 or bf16, ``k_cache`` / ``v_cache [pages, Hkv, page_size, D]`` of the same type (``Hq`` a multiple of
+    ``Hkv``), ``page_table`` int32 ``[B, pages of the longest]``, ``seq_lens`` int32 ``[B]``: tokens in the cache, the new
+    one included; 0 gives a zero row.  What lies behind a sequence's end, in its last page and in its row of the table, is
+    never read.  ``scale`` defaults to ``D ** -0.5``.  Nothing depends on lengths known to the host: a captured call
+    serves whatever lengths the tensor holds at replay.  Pages and lengths out of range raise at the next
+    :func:`check_device_errors`.
+    """
+    word = _index_word(_on_gpu(q, "q"))
+    y = _lib.host().paged_decode(q, k_cache, v_cache, page_table, seq_lens, scale, out, word)
+    if isinstance(y, int):
+        _lib.check(y, "paged_attention_decode", q=tuple(q.shape), cache=tuple(k_cache.shape))
+    return y
+
+
+def attention_prefill(q, k, v, cu_seqlens, *, scale: float | None = None, out=None):
+    """Causal attention within packed sequences: rows ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` are sequence ``b``.
+
+    ``q [T,Hq,D]``, ``k`` and ``v [T,Hkv,D]`` fp16 or bf16, strided views included, ``Hq`` a multiple of ``Hkv``;
+    ``cu_seqlens`` int32 ``[B + 1]``, ascending, at most ``T``.  Returns ``out [T,Hq,D]``; rows that belong to no sequence
+    are left as they are in ``out``, and unspecified without one.  ``scale`` defaults to ``D ** -0.5``.
+    """
+    device = _on_gpu(q, "q")
+    y = _lib.host().attention_prefill(q, k, v, cu_seqlens, scale, out, _index_word(device), _error_word(device).data_ptr())
+    if isinstance(y, int):
+        _lib.check(y, "attention_prefill", q=tuple(q.shape), k=tuple(k.shape))
     return y
