@@ -2,169 +2,529 @@
 //
 //   o_i = sum_{j <= i} exp(s_ij - m_i) v_j / sum_{j <= i} exp(s_ij - m_i),   s_ij = scale q_i . k_j
 //
-// with a running maximum, sum and output over tiles of keys.
+// with a running maximum, sum and output over tiles of 128 keys.  A block works on two tiles of 128 query rows that share
+// their keys and values -- two heads of a group at the same tokens, or 256 tokens of a head -- so that the tensor cores have
+// one tile's products to do while the other tile's exponentials are taken:
+//
+//   warp 0   copies (TMA): queries, then keys and values in turn through a ring
+//   warp 1   tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory
+//   warps 4-7 and 8-11, one group to a tile: a thread has one row; it takes S from tensor memory, the row's maximum, the
+//            exponentials, and leaves P, rounded, where S was
+//
+// The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights stay below
+// that in either type, the sum is in fp32), so most tiles leave O alone.  Bounds: for heads of 128 values a tile's two
+// products take the tensor cores 1024 clocks and its 16384 exponentials as many.
+//
+// What a row may not attend to must not reach it, whatever it holds: scores are replaced where masked, but 0 x NaN is NaN in
+// the product with V.  So before the last tile of a sequence's row the group clears rows of V behind the sequence's end and
+// looks for values that are not finite; where there are any, the threads add that tile's product up themselves.
 #include "attention.cuh"
 
 namespace mp {
 namespace {
 
 using namespace attn;
+using namespace tc;
 
-constexpr int kRowsPerBlock = 64, kKeys = 64, kThreads = 128;
+constexpr int kTile = 128;                     // query rows of a tile and keys of a step
+// Four warps of copies, products and none of either, and two groups of four.  Registers: the block starts with 168 a thread,
+// 64512 in all; the first four warps give back what the others take, 128 x 56 + 256 x 224 = 64512.
+constexpr int kWarps = 12, kThreads = 32 * kWarps;
+constexpr int kFewRegisters = 56, kManyRegisters = 224;
+constexpr int kTmemCols = 512;
+constexpr float kGrowth = 8.0f;                // log2 of how far weights may exceed 1
+
+template <int DP>
+struct Prefill {
+  static constexpr int kBoxes = DP / 64;                       // copies of 64 columns
+  static constexpr int kTileBytes = kTile * DP * 2;
+  static constexpr int kStages = DP == 64 ? 8 : 5;
+  static constexpr int kBarBytes = 256;
+  static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + kBarBytes + 1024;
+};
 
 struct PrefillParams {
-  HeadRows q, k, v;
   const int* cu_seqlens;
   char* out;
   int* index_word;
+  int* error_word;
   int tokens, batch, q_heads, group, dim;
-  float scale_log2;
+  int pair_heads;                              // the block's two tiles: 1 two heads, 0 two tiles of a head
+  int slots, per_slot;                         // numbers of row tiles, and the items of each
+  float scale_log2;                            // |scale| log2 e
+  int negative;                                // scale < 0
+  int q_swap, kv_swap, v_swap;                 // which of token and head is the tensor map's dimension 1
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) prefill_kernel(const PrefillParams p) {
-  extern __shared__ __align__(128) char smem[];
-  chain_wait();
-  chain_release();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // Tile numbers: sequence b has those from cu[b] / 64 + b on, which is room for all its tiles, so that the sequence of a
-  // tile is found without the sum of the others'.
-  const int number = blockIdx.x;
-  int lo = 0, hi = p.batch;                     // first number of lo <= number < first number of hi
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (__ldg(p.cu_seqlens + mid) / kRowsPerBlock + mid <= number) lo = mid; else hi = mid;
-  }
-  const int begin = __ldg(p.cu_seqlens + lo), end = __ldg(p.cu_seqlens + lo + 1);
-  if (begin < 0 || end < begin || end > p.tokens) {
-    if (p.index_word) *p.index_word = kBadIndex;
-    return;
-  }
-  const int row_begin = (number - begin / kRowsPerBlock - lo) * kRowsPerBlock, len = end - begin;
-  if (row_begin < 0 || row_begin >= len) return;
-  const int head = blockIdx.y, kv = head / p.group;
-  const int row0 = row_begin + warp * 16 + (lane >> 2), col0 = (lane & 3) * 2;
-  uint32_t qf[DP / 16][4];
-  const char* q = p.q.data + begin * p.q.token_stride + head * p.q.head_stride;
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// one column of the warp's 32 lanes, complete on return
+__device__ __forceinline__ uint32_t tmem_ld_column(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(taddr) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Eight values: true where one is infinite or NaN (all exponent bits set).
+template <typename T> __device__ __forceinline__ bool any_not_finite(const uint4& v) {
+  constexpr uint32_t kExp = sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u;
+  bool bad = false;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = row0 + (j & 1) * 8, c = k * 16 + col0 + (j >> 1) * 8;
-      qf[k][j] = r >= len || c >= p.dim ? 0u : __ldg(reinterpret_cast<const unsigned int*>(q + r * p.q.token_stride + c * 2));
+  for (int i = 0; i < 4; ++i) bad = bad || (w[i] & kExp) == kExp || ((w[i] >> 16) & kExp) == kExp;
+  return bad;
+}
+
+// Descriptor of V as the B operand [dims x keys] whose rows in memory are keys (128 bytes of 64 dims, 128-byte swizzle):
+// eight keys are 1024 bytes apart, the next 64 dims one box of the tile.
+__device__ __forceinline__ uint64_t umma_desc_rows_sw128(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>((kTile * 128) >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+// What a block does next.
+struct Work {
+  int begin, len;              // the sequence
+  int row[2], head[2];         // the two tiles' first rows within it, and their heads
+  int steps[2];                // tiles of keys; 0: there is no such tile
+  int kv;
+};
+
+__device__ __forceinline__ bool next_work(const PrefillParams& p, int& item, Work& w) {
+  const int rows = p.pair_heads ? kTile : 2 * kTile, total = p.slots * p.per_slot;
+  for (; item < total; item += gridDim.x) {
+    // Numbers of row tiles: sequence b has those from cu[b] / rows + b on, which is room for all its tiles, so that a tile's
+    // sequence is found without the others' sum.  The last rows of a sequence, which take longest, come first.
+    const int number = p.slots - 1 - item / p.per_slot, at = item % p.per_slot;
+    int lo = 0, hi = p.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (__ldg(p.cu_seqlens + mid) / rows + mid <= number) lo = mid; else hi = mid;
     }
-  const char* k_rows = p.k.data + begin * p.k.token_stride + kv * p.k.head_stride;
-  const char* v_rows = p.v.data + begin * p.v.token_stride + kv * p.v.head_stride;
-  constexpr int kPieces = DP / 8, kSide = kKeys * DP * 2;
-  const uint32_t base = tc::smem_u32(smem);
-  auto load = [&](int tile) {
-    const uint32_t dst = base + (tile & 1) * 2 * kSide;
-    for (int i = threadIdx.x; i < kKeys * kPieces; i += kThreads) {
-      const int row = i / kPieces, piece = i - row * kPieces, key = tile * kKeys + row;
-      const bool valid = key < len && piece * 8 < p.dim;
-      const long long r = valid ? key : 0;
-      const int c = valid ? piece * 16 : 0;
-      copy16_async(dst + piece_at<DP>(row, piece), k_rows + r * p.k.token_stride + c, valid);
-      copy16_async(dst + kSide + piece_at<DP>(row, piece), v_rows + r * p.v.token_stride + c, valid);
+    w.begin = __ldg(p.cu_seqlens + lo);
+    const int end = __ldg(p.cu_seqlens + lo + 1);
+    if (w.begin < 0 || end < w.begin || end > p.tokens) {
+      if (p.index_word) *p.index_word = kBadIndex;
+      continue;
     }
-    copies_commit();
-  };
-  constexpr int kNT = DP / 8;
-  float o[kNT][4];
+    w.len = end - w.begin;
+    const int row = (number - w.begin / rows - lo) * rows;
+    if (row < 0 || row >= w.len) continue;
+    w.row[0] = row;
+    w.row[1] = p.pair_heads ? row : row + kTile;
+    w.head[0] = p.pair_heads ? 2 * at : at;
+    w.head[1] = p.pair_heads ? 2 * at + 1 : at;
+    w.kv = w.head[0] / p.group;
 #pragma unroll
-  for (int n = 0; n < kNT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-  float m[2] = {kNegInf, kNegInf}, sum[2] = {0.0f, 0.0f};
-  const int tiles = (min(row_begin + kRowsPerBlock, len) + kKeys - 1) / kKeys;
-  load(0);
-  for (int t = 0; t < tiles; ++t) {
-    if (t + 1 < tiles) load(t + 1); else copies_commit();
-    copies_wait<1>();
-    __syncthreads();
-    const uint32_t tile_k = base + (t & 1) * 2 * kSide, tile_v = tile_k + kSide;
-    float s[kKeys / 8][4];
-#pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-      for (int n = 0; n < kKeys / 16; ++n) {
-        uint32_t b[4];
-        ldmatrix_x4(b, tile_k + piece_at<DP>(n * 16 + (lane & 7) + (lane >> 4) * 8, k * 2 + ((lane >> 3) & 1)));
-        mma_16816<T>(s[2 * n], qf[k], b[0], b[1]);
-        mma_16816<T>(s[2 * n + 1], qf[k], b[2], b[3]);
-      }
-    float keep[2], ref[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float top = kNegInf;
-#pragma unroll
-      for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float& v = s[n][2 * h + j];
-          v = t * kKeys + n * 8 + col0 + j <= row0 + 8 * h ? v * p.scale_log2 : kNegInf;
-          top = fmaxf(top, v);
-        }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float now = fmaxf(m[h], top);
-      ref[h] = now == kNegInf ? 0.0f : now;
-      keep[h] = exp2_fast(m[h] - ref[h]);
-      m[h] = now;
-      sum[h] *= keep[h];
-    }
-    uint32_t pf[kKeys / 16][4];
-#pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float e0 = exp2_fast(s[n][2 * h] - ref[h]), e1 = exp2_fast(s[n][2 * h + 1] - ref[h]);
-        sum[h] += e0 + e1;
-        pf[n >> 1][(n & 1) * 2 + h] = pack2<T>(e0, e1);
-      }
-#pragma unroll
-    for (int n = 0; n < kNT; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[n][j] *= keep[j >> 1];
-#pragma unroll
-    for (int k = 0; k < kKeys / 16; ++k)
-#pragma unroll
-      for (int n = 0; n < kNT / 2; ++n) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(b, tile_v + piece_at<DP>(k * 16 + (lane & 15), n * 2 + (lane >> 4)));
-        mma_16816<T>(o[2 * n], pf[k], b[0], b[1]);
-        mma_16816<T>(o[2 * n + 1], pf[k], b[2], b[3]);
-      }
-    __syncthreads();
+    for (int i = 0; i < 2; ++i) w.steps[i] = w.row[i] < w.len ? w.row[i] / kTile + 1 : 0;
+    return true;
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-    const float inv = 1.0f / sum[h];
-    const int r = row0 + 8 * h;
-    if (r >= len) continue;
-    char* dst = p.out + ((static_cast<long long>(begin) + r) * p.q_heads + head) * p.dim * 2;
-#pragma unroll
-    for (int n = 0; n < kNT; ++n) {
-      const int c = n * 8 + col0;
-      if (c < p.dim) *reinterpret_cast<uint32_t*>(dst + c * 2) = pack2<T>(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
-    }
-  }
+  return false;
 }
 
 template <typename T, int DP>
-int launch_prefill(const PrefillParams& p, cudaStream_t st) {
-  const int smem = 4 * kKeys * DP * 2;
+__global__ void __launch_bounds__(kThreads, 1)
+prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+               const __grid_constant__ CUtensorMap map_v, const PrefillParams p) {
+  using C = Prefill<DP>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (2 + C::kStages) * C::kTileBytes);
+  const uint32_t q_tile = smem_u32(smem), ring = q_tile + 2 * C::kTileBytes;
+  const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * C::kStages, q_full = kv_empty + 8 * C::kStages,
+                 q_empty = q_full + 16, s_full = q_empty + 16, p_ready = s_full + 16, o_done = p_ready + 16, scanned = o_done + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 12);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  // [tile][item's parity]: the last product of the tile's item is not the MMA's
+  volatile int* odd_values = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  static_assert(8 * (2 * C::kStages + 12) + 24 <= C::kBarBytes, "");
+
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(kv_full + 8 * s, 1);
+      mbar_init(kv_empty + 8 * s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + 8 * i, 1);
+      mbar_init(q_empty + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_ready + 8 * i, 4);
+      mbar_init(o_done + 8 * i, 1);
+      mbar_init(scanned + 8 * i, 4);
+      odd_values[2 * i] = odd_values[2 * i + 1] = 0;
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&map_q);
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  chain_wait();
+  chain_release();
+
+  int item = blockIdx.x;
+  Work w;
+  // (each side's code hangs below its own setmaxnreg, or the compiler holds all of it to the smaller number)
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    if (warp == 0 && elect_one()) {
+      int load = 0;                            // copies of keys and values so far
+      uint32_t q_phase[2] = {1, 1};
+      bool ok = true;
+      auto copy = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int swap, int head, int token) {
+#pragma unroll
+        for (int b = 0; b < C::kBoxes; ++b)
+          tma_load_3d(dst + b * kTile * 128, map, bar, b * 64, swap ? token : head, swap ? head : token);
+      };
+      auto next_slot = [&](uint32_t& dst, uint32_t& bar) {
+        const int s = load % C::kStages;
+        dst = ring + s * C::kTileBytes;
+        bar = kv_full + 8 * s;
+        if (!mbar_wait(kv_empty + 8 * s, ((load / C::kStages) & 1) ^ 1, abort_flag)) return false;
+        mbar_arrive_expect_tx(bar, C::kTileBytes);
+        ++load;
+        return true;
+      };
+      for (; ok && next_work(p, item, w); item += gridDim.x) {
+        const int steps = max(w.steps[0], w.steps[1]);
+        uint32_t dst, bar;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!w.steps[i]) continue;
+          if (!mbar_wait(q_empty + 8 * i, q_phase[i], abort_flag)) { ok = false; break; }
+          q_phase[i] ^= 1;
+          mbar_arrive_expect_tx(q_full + 8 * i, C::kTileBytes);
+          copy(q_tile + i * C::kTileBytes, &map_q, q_full + 8 * i, p.q_swap, w.head[i], w.begin + w.row[i]);
+          if (i == 0) {
+            if (!next_slot(dst, bar)) { ok = false; break; }
+            copy(dst, &map_k, bar, p.kv_swap, w.kv, w.begin);
+          }
+        }
+        for (int j = 0; ok && j < steps; ++j) {
+          if (j) {
+            if (!next_slot(dst, bar)) { ok = false; break; }
+            copy(dst, &map_k, bar, p.kv_swap, w.kv, w.begin + j * kTile);
+          }
+          if (!next_slot(dst, bar)) { ok = false; break; }
+          copy(dst, &map_v, bar, p.v_swap, w.kv, w.begin + j * kTile);
+        }
+      }
+    }
+    if (warp == 1 && elect_one()) {
+      constexpr uint32_t kFormats = kIdescDFormatF32 | (__is_same(T, __half) ? 0u : (1u << 7) | (1u << 10));
+      constexpr uint32_t kIdescQK = umma_idesc(kFormats, kTile, kTile);
+      constexpr uint32_t kIdescPV = umma_idesc(kFormats, kTile, DP) | (1u << 16);      // B's rows in memory are K
+      int load = 0;
+      uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, parity[2] = {0, 0};
+      bool ok = true;
+      auto full = [&](int n) { return mbar_wait(kv_full + 8 * (n % C::kStages), (n / C::kStages) & 1, abort_flag); };
+      auto scores = [&](int i, int n) {        // S_i = Q_i K^T with the keys of copy n
+        const uint64_t a = umma_desc_k_sw128(q_tile + i * C::kTileBytes);
+        const uint64_t b = umma_desc_k_sw128(ring + (n % C::kStages) * C::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t at = (k >> 2) * ((kTile * 128) >> 4) + 2 * (k & 3);
+          umma_ss(tmem + i * kTile, a + at, b + at, kIdescQK, k != 0);
+        }
+        umma_commit(s_full + 8 * i);
+      };
+      for (; ok && next_work(p, item, w); item += gridDim.x) {
+        const int steps = max(w.steps[0], w.steps[1]);
+        if (!full(load)) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!w.steps[i]) continue;
+          if (!mbar_wait(q_full + 8 * i, q_phase[i], abort_flag)) { ok = false; break; }
+          q_phase[i] ^= 1;
+          tcgen05_fence_after();
+          scores(i, load);
+          if (w.steps[i] == 1) umma_commit(q_empty + 8 * i);
+        }
+        umma_commit(kv_empty + 8 * (load % C::kStages));
+        for (int j = 0; ok && j < steps; ++j) {
+          const int nv = load + 2 * j + 1, nk = nv + 1;       // the copies of this step's values and the next one's keys
+          if (!full(nv)) { ok = false; break; }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (j >= w.steps[i]) continue;
+            if (!mbar_wait(p_ready + 8 * i, p_phase[i], abort_flag)) { ok = false; break; }
+            p_phase[i] ^= 1;
+            tcgen05_fence_after();
+            if (j + 1 < w.steps[i] || !odd_values[2 * i + parity[i]]) {
+              const uint64_t b = umma_desc_rows_sw128(ring + (nv % C::kStages) * C::kTileBytes);
+#pragma unroll
+              for (int k = 0; k < kTile / 16; ++k)
+                umma_ts(tmem + 2 * kTile + i * DP, tmem + i * kTile + k * 8, b + k * ((16 * 128) >> 4), kIdescPV, j != 0 || k != 0);
+            }
+            umma_commit(o_done + 8 * i);
+            if (j + 1 == w.steps[i]) {
+              parity[i] ^= 1;
+            } else {
+              if (!full(nk)) { ok = false; break; }
+              tcgen05_fence_after();
+              scores(i, nk);
+              if (j + 2 == w.steps[i]) umma_commit(q_empty + 8 * i);
+            }
+          }
+          umma_commit(kv_empty + 8 * (nv % C::kStages));
+          if (j + 1 < steps) umma_commit(kv_empty + 8 * (nk % C::kStages));
+        }
+        load += 2 * steps;
+      }
+    }
+  } else {
+    // ---- one row of tile i to a thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    const int i = warp >= 8, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_tmem = tmem + lanes + i * kTile, o_tmem = tmem + lanes + 2 * kTile + i * DP;
+    uint32_t s_phase = 0, o_phase = 0, scan_phase = 0;         // o_phase: of the next product to complete
+    int load = 0;
+    bool ok = true;
+    auto wait_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
+    for (; ok && next_work(p, item, w); item += gridDim.x) {
+      const int steps = i ? w.steps[1] : w.steps[0], row_begin = i ? w.row[1] : w.row[0], head = i ? w.head[1] : w.head[0];
+      const int first_load = load;
+      load += 2 * max(w.steps[0], w.steps[1]);
+      if (!steps) continue;
+      float m = kNegInf, sum = 0.0f;
+      for (int j = 0; j < steps; ++j) {
+        if (!wait_all(s_full + 8 * i, s_phase)) { ok = false; break; }
+        s_phase ^= 1;
+        tcgen05_fence_after();
+        const bool last = j + 1 == steps;
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_tmem + 32 * c, s[c]);
+        tmem_ld_wait();
+        auto value = [&](int c) -> uint32_t& { return s[c >> 5][c & 31]; };
+        if (p.negative) {
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) value(c) ^= 0x80000000u;
+        }
+        if (last) {
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) value(c) = c <= row ? value(c) : __float_as_uint(kNegInf);
+        }
+        float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(value(c)));
+        const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2);
+        // products of this tile that are complete: j (the next to complete is number j + 1)
+        if (j == 0) {
+          m = now;
+        } else if (__any_sync(0xffffffffu, now > m + kGrowth)) {
+          if (!wait_all(o_done + 8 * i, o_phase ^ 1)) { ok = false; break; }      // product j
+          tcgen05_fence_after();
+          const float keep = now == kNegInf ? 1.0f : exp2_fast(m - now);
+          sum *= keep;
+          m = now;
+#pragma unroll
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(o_tmem + 32 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+            tmem_st_32x32(o_tmem + 32 * c, o);
+          }
+        }
+        o_phase ^= 1;
+        const float ref = m == kNegInf ? 0.0f : m;
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int c = h * 64 + 2 * e;
+            const float a = exp2_fast(fmaf(__uint_as_float(value(c)), p.scale_log2, -ref));
+            const float b = exp2_fast(fmaf(__uint_as_float(value(c + 1)), p.scale_log2, -ref));
+            part[e & 1] += a;
+            part[2 + (e & 1)] += b;
+            packed[e] = pack2<T>(a, b);
+          }
+          tmem_st_32x32(s_tmem + 32 * h, packed);
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        if (last) {
+          // ---- V's rows behind the sequence's end, and values that are not finite
+          const int n = first_load + 2 * j + 1, valid = w.len - j * kTile;
+          if (!wait_all(kv_full + 8 * (n % C::kStages), (n / C::kStages) & 1)) { ok = false; break; }
+          const uint32_t tile_v = ring + (n % C::kStages) * C::kTileBytes;
+          bool odd = false;
+#pragma unroll
+          for (int b = 0; b < C::kBoxes; ++b)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const int r = c * 16 + quarter * 4 + (lane >> 3);           // 16 rows of eight pieces
+              const uint32_t at = tile_v + b * kTile * 128 + r * 128 + (lane & 7) * 16;
+              if (r < valid) odd = odd || any_not_finite<T>(lds16(at));
+              else asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0u) : "memory");
+            }
+          if (valid < kTile) fence_proxy_async_smem();
+          if (__any_sync(0xffffffffu, odd) && lane == 0) odd_values[2 * i + scan_phase] = 1;
+          // (whoever read the other one, for the item before, has done so: that item's last product is complete)
+          if (quarter == 0 && lane == 0) odd_values[2 * i + (scan_phase ^ 1)] = 0;
+          mbar_arrive_warp(scanned + 8 * i, lane);
+          if (!wait_all(scanned + 8 * i, scan_phase)) { ok = false; break; }
+          scan_phase ^= 1;
+          if (odd_values[2 * i + (scan_phase ^ 1)]) {
+            // this row's product with the keys it attends to, 32 columns at a time
+            tmem_st_wait();
+            if (j > 0) {
+              if (!wait_all(o_done + 8 * i, o_phase)) { ok = false; break; }      // product j, of the tile before
+              tcgen05_fence_after();
+            }
+            for (int d0 = 0; d0 < DP; d0 += 32) {
+              uint32_t o[32];
+              if (j > 0) {
+                tmem_ld_32x32(o_tmem + d0, o);
+                tmem_ld_wait();
+              } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0u;
+              }
+              for (int c = 0; c < kTile; c += 2) {
+                const float2 pair = unpack2<T>(tmem_ld_column(s_tmem + c / 2));
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  if (c + k > row) continue;
+                  const float weight = k ? pair.y : pair.x;
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const uint4 v = lds16(tile_v + (d0 >> 6) * kTile * 128 + (c + k) * 128 + ((((d0 & 63) / 8 + e) ^ ((c + k) & 7)) << 4));
+                    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                      const float2 y = unpack2<T>(words[x]);
+                      uint32_t &o0 = o[e * 8 + 2 * x], &o1 = o[e * 8 + 2 * x + 1];
+                      o0 = __float_as_uint(fmaf(weight, y.x, __uint_as_float(o0)));
+                      o1 = __float_as_uint(fmaf(weight, y.y, __uint_as_float(o1)));
+                    }
+                  }
+                }
+              }
+              tmem_st_32x32(o_tmem + d0, o);
+            }
+          }
+        }
+        tmem_st_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready + 8 * i);
+      }
+      if (!ok) break;
+      // ---- the row's result
+      if (!wait_all(o_done + 8 * i, o_phase ^ 1)) { ok = false; break; }
+      tcgen05_fence_after();
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int at = row_begin + row;
+      char* dst = p.out + ((static_cast<long long>(w.begin) + at) * p.q_heads + head) * p.dim * 2;
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld_32x32(o_tmem + 32 * c, o);
+        tmem_ld_wait();
+        if (at < w.len) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t word[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              word[x] = pack2<T>(__uint_as_float(o[e * 8 + 2 * x]) * inv, __uint_as_float(o[e * 8 + 2 * x + 1]) * inv);
+            if (c * 32 + e * 8 < p.dim)
+              *reinterpret_cast<uint4*>(dst + (c * 32 + e * 8) * 2) = make_uint4(word[0], word[1], word[2], word[3]);
+          }
+        }
+      }
+      tcgen05_fence_before();
+    }
+  }
+
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0 && p.error_word) atomicExch(p.error_word, 1);
+    // give copies and products still in flight time to end before their memory goes away
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// [T, heads, D] as a tensor of three dimensions, the one of token and head with the smaller stride first; boxes of one head,
+// 128 tokens and 64 columns.
+int head_map(CUtensorMap* map, int dtype, const HeadRows& r, int tokens, int heads, int dim, int* swap) {
+  if ((r.token_stride == 0 && tokens > 1) || (r.head_stride == 0 && heads > 1)) return MP_ERR_UNSUPPORTED;
+  const uint64_t token = tokens > 1 ? r.token_stride : 16, head = heads > 1 ? r.head_stride : 16;
+  *swap = token < head;
+  const uint64_t dims[3] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(*swap ? tokens : heads),
+                            static_cast<uint64_t>(*swap ? heads : tokens)};
+  const uint64_t strides[2] = {*swap ? token : head, *swap ? head : token};
+  const uint32_t box[3] = {64, *swap ? static_cast<uint32_t>(kTile) : 1u, *swap ? 1u : static_cast<uint32_t>(kTile)};
+  return encode_tensor_map_3d(map, dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r.data, dims,
+                              strides, box);
+}
+
+template <typename T, int DP>
+int launch_prefill(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const PrefillParams& p, cudaStream_t st) {
+  using C = Prefill<DP>;
   static thread_local int configured_device = -1;
   int device = 0;
   MP_CUDA_TRY(cudaGetDevice(&device));
   if (configured_device != device) {
-    MP_CUDA_TRY(cudaFuncSetAttribute(prefill_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    MP_CUDA_TRY(cudaFuncSetAttribute(prefill_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     configured_device = device;
   }
-  const dim3 grid(p.tokens / kRowsPerBlock + p.batch, p.q_heads);
-  return launch_chained(prefill_kernel<T, DP>, grid, dim3(kThreads), smem, st, p);
+  const long long items = static_cast<long long>(p.slots) * p.per_slot;
+  const int grid = static_cast<int>(items < kSmCount ? items : kSmCount);
+  return launch_chained(prefill_kernel<T, DP>, dim3(grid), dim3(kThreads), C::kSmem, st, q, k, v, p);
 }
 
 }  // namespace
@@ -174,23 +534,33 @@ extern "C" int mp_attention_prefill(int dtype, const mp_head_rows* q, const mp_h
                                     int Hq, int Hkv, int D, const void* cu_seqlens_i32, int B, float scale, void* out,
                                     int* index_word, int* error_word, mp_stream_t stream) {
   using namespace mp;
-  PrefillParams p{};
+  HeadRows qr, kr, vr;
   int rc;
-  if ((rc = check_head_rows(q, D, &p.q)) || (rc = check_head_rows(k, D, &p.k)) || (rc = check_head_rows(v, D, &p.v))) return rc;
+  if ((rc = check_head_rows(q, D, &qr)) || (rc = check_head_rows(k, D, &kr)) || (rc = check_head_rows(v, D, &vr))) return rc;
   if (!cu_seqlens_i32 || !out || T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0) return MP_ERR_INVALID_ARG;
   if ((dtype != 0 && dtype != 1) || Hq % Hkv || Hq > 65535) return MP_ERR_UNSUPPORTED;
   if (!aligned(out, 16)) return MP_ERR_ALIGNMENT;
+  PrefillParams p{};
   p.cu_seqlens = static_cast<const int*>(cu_seqlens_i32);
   p.out = static_cast<char*>(out);
   p.index_word = index_word;
+  p.error_word = error_word;
   p.tokens = T;
   p.batch = B;
   p.q_heads = Hq;
   p.group = Hq / Hkv;
   p.dim = D;
-  p.scale_log2 = scale * attn::kLog2e;
-  (void)error_word;
+  p.pair_heads = p.group % 2 == 0;
+  p.slots = T / (p.pair_heads ? kTile : 2 * kTile) + B;
+  p.per_slot = p.pair_heads ? Hq / 2 : Hq;
+  if (static_cast<long long>(p.slots) * p.per_slot > 0x7fff0000LL) return MP_ERR_UNSUPPORTED;
+  p.scale_log2 = fmaxf(fabsf(scale) * attn::kLog2e, 1e-30f);      // masked scores stay minus infinity with a scale of 0 too
+  p.negative = scale < 0.0f;
+  CUtensorMap mq, mk, mv;
+  if ((rc = head_map(&mq, dtype, qr, T, Hq, D, &p.q_swap)) || (rc = head_map(&mk, dtype, kr, T, Hkv, D, &p.kv_swap)) ||
+      (rc = head_map(&mv, dtype, vr, T, Hkv, D, &p.v_swap)))
+    return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (D <= 64) return dtype == 0 ? launch_prefill<__half, 64>(p, st) : launch_prefill<__nv_bfloat16, 64>(p, st);
-  return dtype == 0 ? launch_prefill<__half, 128>(p, st) : launch_prefill<__nv_bfloat16, 128>(p, st);
+  if (D <= 64) return dtype == 0 ? launch_prefill<__half, 64>(mq, mk, mv, p, st) : launch_prefill<__nv_bfloat16, 64>(mq, mk, mv, p, st);
+  return dtype == 0 ? launch_prefill<__half, 128>(mq, mk, mv, p, st) : launch_prefill<__nv_bfloat16, 128>(mq, mk, mv, p, st);
 }

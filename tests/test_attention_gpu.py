@@ -243,6 +243,49 @@ def test_prefill_rows_of_no_sequence_are_left_alone():
     assert torch.equal(out[:10], before[:10]) and torch.equal(out[271:], before[271:])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 128), (3, 1, 64), (2, 2, 80)])
+@pytest.mark.parametrize("at", [5, 127, 128, 200, 300, 399])
+def test_prefill_infinite_and_nan_values_reach_only_later_rows(at, h, hk, d, dtype):
+    """Values (and keys) of a token that are not finite: the rows in front of it are those of a clean token."""
+    ends = [0, 37, 437, 500]
+    q, k, v = (x.contiguous() for x in heads(500, h, hk, d, dtype, 6))
+    token = ends[1] + at
+    v[token, 0, 3], v[token, 0, d - 1] = float("inf"), float("nan")
+    clean = v.clone()
+    clean[token, 0, 3], clean[token, 0, d - 1] = 0, 0
+    cu = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    got = ops.attention_prefill(q, k, v, cu)
+    want, tol = ref.prefill(q, k, clean, ends)
+    hit = torch.zeros_like(want, dtype=torch.bool)
+    hit[token:ends[2], :h // hk, 3] = hit[token:ends[2], :h // hk, d - 1] = True
+    ref.assert_close(got[~hit], want[~hit], tol[~hit])
+    assert (got[token:ends[2], :h // hk, 3] == float("inf")).all() and got[token:ends[2], :h // hk, d - 1].isnan().all()
+    k[token, 0] = float("nan")
+    got = ops.attention_prefill(q, k, clean, cu)
+    hit[token:ends[2], :h // hk] = True
+    ref.assert_close(got[~hit], want[~hit], tol[~hit])
+    assert got[token:ends[2], :h // hk].isnan().all()
+    ops.check_device_errors()
+
+
+def test_prefill_operands_of_other_strides():
+    """Heads first in memory, padded rows, one head of keys for all by expansion, a slice of heads."""
+    t, h, d, ends = 410, 4, 64, [0, 300, 410]
+    q, k = randn(h, t, d, seed=1).transpose(0, 1), randn(2, t, d + 8, seed=2)[..., :d].transpose(0, 1)
+    v = randn(t, 7, d, seed=3)[:, 2:6:2]
+    cu = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    want, tol = ref.prefill(q, k, v, ends)
+    ref.assert_close(ops.attention_prefill(q, k, v, cu), want, tol)
+    one = k[:, :1].expand(t, 4, d)
+    try:
+        got = ops.attention_prefill(q, one, one, cu)
+    except _lib.MindPipeKernelError:                              # refused, not wrong
+        return
+    want, tol = ref.prefill(q, one, one, ends)
+    ref.assert_close(got, want, tol)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.2, 5.0])
 def test_prefill_scales(scale):
     ends = [0, 333, 600]
