@@ -43,6 +43,11 @@ struct Prefill {
   static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + kBarBytes + 1024;
 };
 
+struct MapOrder {
+  int token_first;                             // the tensor map's dimensions are D, token, head; else D, head, token
+  int one_head;                                // all heads are the same rows
+};
+
 struct PrefillParams {
   const int* cu_seqlens;
   char* out;
@@ -53,7 +58,7 @@ struct PrefillParams {
   int slots, per_slot;                         // numbers of row tiles, and the items of each
   float scale_log2;                            // |scale| log2 e
   int negative;                                // scale < 0
-  int q_swap, kv_swap, v_swap;                 // which of token and head is the tensor map's dimension 1
+  MapOrder q_order, k_order, v_order;
 };
 
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -213,10 +218,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       int load = 0;                            // copies of keys and values so far
       uint32_t q_phase[2] = {1, 1};
       bool ok = true;
-      auto copy = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int swap, int head, int token) {
+      auto copy = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, const MapOrder& order, int head, int token) {
+        if (order.one_head) head = 0;
 #pragma unroll
         for (int b = 0; b < C::kBoxes; ++b)
-          tma_load_3d(dst + b * kTile * 128, map, bar, b * 64, swap ? token : head, swap ? head : token);
+          tma_load_3d(dst + b * kTile * 128, map, bar, b * 64, order.token_first ? token : head, order.token_first ? head : token);
       };
       auto next_slot = [&](uint32_t& dst, uint32_t& bar) {
         const int s = load % C::kStages;
@@ -236,19 +242,19 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           if (!mbar_wait(q_empty + 8 * i, q_phase[i], abort_flag)) { ok = false; break; }
           q_phase[i] ^= 1;
           mbar_arrive_expect_tx(q_full + 8 * i, C::kTileBytes);
-          copy(q_tile + i * C::kTileBytes, &map_q, q_full + 8 * i, p.q_swap, w.head[i], w.begin + w.row[i]);
+          copy(q_tile + i * C::kTileBytes, &map_q, q_full + 8 * i, p.q_order, w.head[i], w.begin + w.row[i]);
           if (i == 0) {
             if (!next_slot(dst, bar)) { ok = false; break; }
-            copy(dst, &map_k, bar, p.kv_swap, w.kv, w.begin);
+            copy(dst, &map_k, bar, p.k_order, w.kv, w.begin);
           }
         }
         for (int j = 0; ok && j < steps; ++j) {
           if (j) {
             if (!next_slot(dst, bar)) { ok = false; break; }
-            copy(dst, &map_k, bar, p.kv_swap, w.kv, w.begin + j * kTile);
+            copy(dst, &map_k, bar, p.k_order, w.kv, w.begin + j * kTile);
           }
           if (!next_slot(dst, bar)) { ok = false; break; }
-          copy(dst, &map_v, bar, p.v_swap, w.kv, w.begin + j * kTile);
+          copy(dst, &map_v, bar, p.v_order, w.kv, w.begin + j * kTile);
         }
       }
     }
@@ -499,15 +505,17 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 }
 
 // [T, heads, D] as a tensor of three dimensions, the one of token and head with the smaller stride first; boxes of one head,
-// 128 tokens and 64 columns.
-int head_map(CUtensorMap* map, int dtype, const HeadRows& r, int tokens, int heads, int dim, int* swap) {
-  if ((r.token_stride == 0 && tokens > 1) || (r.head_stride == 0 && heads > 1)) return MP_ERR_UNSUPPORTED;
+// 128 tokens and 64 columns.  Heads that are one and the same in memory become one.
+int head_map(CUtensorMap* map, int dtype, const HeadRows& r, int tokens, int heads, int dim, MapOrder* order) {
+  if (r.head_stride == 0) heads = 1;
   const uint64_t token = tokens > 1 ? r.token_stride : 16, head = heads > 1 ? r.head_stride : 16;
-  *swap = token < head;
-  const uint64_t dims[3] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(*swap ? tokens : heads),
-                            static_cast<uint64_t>(*swap ? heads : tokens)};
-  const uint64_t strides[2] = {*swap ? token : head, *swap ? head : token};
-  const uint32_t box[3] = {64, *swap ? static_cast<uint32_t>(kTile) : 1u, *swap ? 1u : static_cast<uint32_t>(kTile)};
+  order->token_first = token < head;
+  order->one_head = heads == 1;
+  const bool first = order->token_first;
+  const uint64_t dims[3] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(first ? tokens : heads),
+                            static_cast<uint64_t>(first ? heads : tokens)};
+  const uint64_t strides[2] = {first ? token : head, first ? head : token};
+  const uint32_t box[3] = {64, first ? static_cast<uint32_t>(kTile) : 1u, first ? 1u : static_cast<uint32_t>(kTile)};
   return encode_tensor_map_3d(map, dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r.data, dims,
                               strides, box);
 }
@@ -539,6 +547,7 @@ extern "C" int mp_attention_prefill(int dtype, const mp_head_rows* q, const mp_h
   if ((rc = check_head_rows(q, D, &qr)) || (rc = check_head_rows(k, D, &kr)) || (rc = check_head_rows(v, D, &vr))) return rc;
   if (!cu_seqlens_i32 || !out || T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0) return MP_ERR_INVALID_ARG;
   if ((dtype != 0 && dtype != 1) || Hq % Hkv || Hq > 65535) return MP_ERR_UNSUPPORTED;
+  if (T > 1 && (qr.token_stride == 0 || kr.token_stride == 0 || vr.token_stride == 0)) return MP_ERR_UNSUPPORTED;
   if (!aligned(out, 16)) return MP_ERR_ALIGNMENT;
   PrefillParams p{};
   p.cu_seqlens = static_cast<const int*>(cu_seqlens_i32);
@@ -557,8 +566,8 @@ extern "C" int mp_attention_prefill(int dtype, const mp_head_rows* q, const mp_h
   p.scale_log2 = fmaxf(fabsf(scale) * attn::kLog2e, 1e-30f);      // masked scores stay minus infinity with a scale of 0 too
   p.negative = scale < 0.0f;
   CUtensorMap mq, mk, mv;
-  if ((rc = head_map(&mq, dtype, qr, T, Hq, D, &p.q_swap)) || (rc = head_map(&mk, dtype, kr, T, Hkv, D, &p.kv_swap)) ||
-      (rc = head_map(&mv, dtype, vr, T, Hkv, D, &p.v_swap)))
+  if ((rc = head_map(&mq, dtype, qr, T, Hq, D, &p.q_order)) || (rc = head_map(&mk, dtype, kr, T, Hkv, D, &p.k_order)) ||
+      (rc = head_map(&mv, dtype, vr, T, Hkv, D, &p.v_order)))
     return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (D <= 64) return dtype == 0 ? launch_prefill<__half, 64>(mq, mk, mv, p, st) : launch_prefill<__nv_bfloat16, 64>(mq, mk, mv, p, st);

@@ -16,6 +16,9 @@ Two entry points with the reference's names, arguments and error behaviour:
 (``exporters/vllm.py:224-327``: ``*.weight_packed / weight_scale / weight_shape``; the W8A8 exporter
 ``scripts/repro/export_fp16_to_ascend_w8a8_dynamic_probe.py:175-195``: ``*.weight / weight_scale / weight_offset``).
 
+:func:`install_paged_attention` replaces the layers' ``self_attn`` by :class:`~mindpipe_b200.attention.PagedSelfAttention`
+around the projections that are there, quantised or not.
+
 The twins quantise on the GPU, so the model's linears must already live on a CUDA device.
 """
 from __future__ import annotations
@@ -25,6 +28,7 @@ from typing import Iterable
 import torch
 from torch import nn
 
+from .attention import PagedKVCache, PagedSelfAttention, rotary_table
 from .modules import SmoothQuantLinear, SmoothQuantPackedMoeExperts, VllmPackedInt4Linear
 
 _ATTN_PROJ = ("q_proj", "k_proj", "v_proj")
@@ -157,6 +161,45 @@ def quantize_model(model, weight_bits=8, activation_bits=8, weight_quant="per_ch
         raise ValueError(f"Invalid weight_quant: {weight_quant}")
     return quantize_llama_like(model, weight_bits=weight_bits, activation_bits=activation_bits, act_quant=act_quant,
                                quantize_bmm_input=quantize_bmm_input)
+
+
+def install_paged_attention(model: nn.Module, cache: PagedKVCache, *, cos_sin: torch.Tensor | None = None,
+                            max_positions: int | None = None) -> list[str]:
+    """Run the attention of every decoder layer on ``cache``; returns the qualified names that were replaced.
+
+    Works before or after the installers of the linears; ``install_paged_attention`` does not touch them.  The rotation's
+    table is ``cos_sin`` (fp32 ``[positions, rotated]``, cosines then sines) or made from the model's ``rotary_emb``
+    (``inv_freq`` and ``attention_scaling``) for ``max_positions`` positions (default: the config's
+    ``max_position_embeddings``).  Layers whose attention does more than project, rotate and attend -- normalised
+    queries or keys, sliding windows, capped scores -- raise ``ValueError`` before anything is replaced.
+    """
+    layers, prefix = get_blocks(model), _blocks_prefix(model)
+    if len(layers) != cache.pool.shape[0]:
+        raise ValueError(f"the model has {len(layers)} layers, the cache {cache.pool.shape[0]}")
+    if cos_sin is None:
+        rotary = next((m for m in model.modules() if hasattr(m, "inv_freq")), None)
+        if rotary is None:
+            raise ValueError("the model has no rotary_emb with inv_freq: pass cos_sin")
+        kind = getattr(rotary, "rope_type", "default")
+        if kind in ("dynamic", "longrope"):
+            raise ValueError(f"the frequencies of rope type {kind!r} depend on the length: pass cos_sin")
+        limit = max_positions or getattr(getattr(model, "config", None), "max_position_embeddings", None)
+        if limit is None:
+            raise ValueError("pass max_positions")
+        cos_sin = rotary_table(rotary.inv_freq.to(cache.pool.device), int(limit), float(getattr(rotary, "attention_scaling", 1.0)))
+    made = []
+    for i, layer in enumerate(layers):
+        attn, name = getattr(layer, "self_attn", None), f"{prefix}.{i}.self_attn"
+        if attn is None:
+            raise ValueError(f"Unsupported layer layout at {prefix}.{i}: expected .self_attn")
+        for extra in ("q_norm", "k_norm", "sliding_window", "attn_logit_softcapping", "sinks"):
+            if getattr(attn, extra, None) is not None:
+                raise ValueError(f"{name}: {extra} is not part of the paged attention")
+        made.append((layer, name, PagedSelfAttention(attn, cache, i, cos_sin, head_dim=getattr(attn, "head_dim", None),
+                                                     scale=getattr(attn, "scaling", None))))
+    for layer, _, new in made:
+        layer.self_attn = new
+    return [name for _, name, _ in made]
 
 
 _W4_KEYS = ("weight_packed", "weight_scale", "weight_zero_point", "weight_shape", "bias")

@@ -278,12 +278,10 @@ def test_prefill_operands_of_other_strides():
     want, tol = ref.prefill(q, k, v, ends)
     ref.assert_close(ops.attention_prefill(q, k, v, cu), want, tol)
     one = k[:, :1].expand(t, 4, d)
-    try:
-        got = ops.attention_prefill(q, one, one, cu)
-    except _lib.MindPipeKernelError:                              # refused, not wrong
-        return
     want, tol = ref.prefill(q, one, one, ends)
-    ref.assert_close(got, want, tol)
+    ref.assert_close(ops.attention_prefill(q, one, one, cu), want, tol)
+    with pytest.raises(_lib.MindPipeKernelError, match="not supported"):
+        ops.attention_prefill(q, k[:1].expand(t, 2, d), v, cu)    # tokens that are all the same row
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 5.0])
