@@ -7,6 +7,7 @@
 // one tile's products to do while the other tile's exponentials are taken:
 //
 //   warp 0   copies (TMA): queries, then keys and values in turn through a ring
+//   warp 2   plans: which tiles, ahead of the others
 //   warp 1   tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory
 //   warps 4-7 and 8-11, one group to a tile: a thread has one row; it takes S from tensor memory, the row's maximum, the
 //            exponentials, and leaves P, rounded, where S was
@@ -27,19 +28,22 @@ using namespace attn;
 using namespace tc;
 
 constexpr int kTile = 128;                     // query rows of a tile and keys of a step
-// Four warps of copies, products and none of either, and two groups of four.  Registers: the block starts with 168 a thread,
-// 64512 in all; the first four warps give back what the others take, 128 x 56 + 256 x 224 = 64512.
+// Four warps of copies, products, planning and nothing, and two groups of four.  Registers: the block starts with 168 a
+// thread, 64512 in all; the first four warps give back what the others take, 128 x 56 + 256 x 224 = 64512.
 constexpr int kWarps = 12, kThreads = 32 * kWarps;
 constexpr int kFewRegisters = 56, kManyRegisters = 224;
 constexpr int kTmemCols = 512;
 constexpr float kGrowth = 8.0f;                // log2 of how far weights may exceed 1
+constexpr int kMultipliedEvery = 4;            // one pair of exponentials in so many by multiplications
+constexpr int kAhead = 4;                      // items that the planning warp is ahead
+constexpr int kSortedBatch = 256;              // sequences whose tiles are taken longest first
 
 template <int DP>
 struct Prefill {
   static constexpr int kBoxes = DP / 64;                       // copies of 64 columns
   static constexpr int kTileBytes = kTile * DP * 2;
   static constexpr int kStages = DP == 64 ? 8 : 5;
-  static constexpr int kBarBytes = 256;
+  static constexpr int kBarBytes = 512;
   static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + kBarBytes + 1024;
 };
 
@@ -98,14 +102,66 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   return v;
 }
 
-// Eight values: true where one is infinite or NaN (all exponent bits set).
-template <typename T> __device__ __forceinline__ bool any_not_finite(const uint4& v) {
-  constexpr uint32_t kExp = sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u;
-  bool bad = false;
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// Eight values times zero, added to a pair: NaN from the first value on that is infinite or NaN.
+template <typename T> struct Pair;
+template <> struct Pair<__half> { using type = __half2; };
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <typename T> __device__ __forceinline__ uint32_t add_zeros(uint32_t acc, const uint4& v) {
+  using P = typename Pair<T>::type;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w}, zero = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad = bad || (w[i] & kExp) == kExp || ((w[i] >> 16) & kExp) == kExp;
-  return bad;
+  for (int i = 0; i < 4; ++i)
+    acc = bits(__hfma2(*reinterpret_cast<const P*>(&w[i]), *reinterpret_cast<const P*>(&zero), *reinterpret_cast<P*>(&acc)));
+  return acc;
+}
+
+// Larger of three, NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Pairs of fp32 values in one instruction.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of a pair by multiplications: x = n + f with n the nearest integer, 2^f by a polynomial of degree 5 (minimax on
+// [-1/2, 1/2], found by exchange; relative error 2^-23.6), n added to the exponent.  x is at most 2^7; below -127 it counts
+// as -127, which gives 0.  The exponential unit takes 16 values a clock and SM, the tensor cores a product of 128 x 128 x 128
+// in the time of 8192: a share of them taken here shortens a tile's turn.  (A NaN does not come through: see the maximum.)
+__device__ __forceinline__ void exp2_pair(F2 x, float& a, float& b) {
+  constexpr float kMagic = 12582912.0f;        // 1.5 * 2^23: added, the sum's low bits are the nearest integer
+  float x0, x1;
+  split(x, x0, x1);
+  x = f2(fmaxf(x0, -127.0f), fmaxf(x1, -127.0f));
+  const F2 t = add2(x, f2(kMagic, kMagic));
+  const F2 f = add2(x, fma2(t, f2(-1.0f, -1.0f), f2(kMagic, kMagic)));
+  F2 r = f2(1.3276472454890609e-3f, 1.3276472454890609e-3f);
+  r = fma2(r, f, f2(9.675540961325169e-3f, 9.675540961325169e-3f));
+  r = fma2(r, f, f2(5.550713092088699e-2f, 5.550713092088699e-2f));
+  r = fma2(r, f, f2(0.24022120237350464f, 0.24022120237350464f));
+  r = fma2(r, f, f2(0.6931469440460205f, 0.6931469440460205f));
+  r = fma2(r, f, f2(1.0000001192092896f, 1.0000001192092896f));
+  float t0, t1;
+  split(t, t0, t1);
+  split(r, a, b);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
 
 // Descriptor of V as the B operand [dims x keys] whose rows in memory are keys (128 bytes of 64 dims, 128-byte swizzle):
@@ -120,7 +176,7 @@ __device__ __forceinline__ uint64_t umma_desc_rows_sw128(uint32_t smem_addr) {
   return d;
 }
 
-// What a block does next.
+// What a block does next: one tile's queries of a sequence, or none (no steps).
 struct Work {
   int begin, len;              // the sequence
   int row[2], head[2];         // the two tiles' first rows within it, and their heads
@@ -128,37 +184,96 @@ struct Work {
   int kv;
 };
 
-__device__ __forceinline__ bool next_work(const PrefillParams& p, int& item, Work& w) {
-  const int rows = p.pair_heads ? kTile : 2 * kTile, total = p.slots * p.per_slot;
-  for (; item < total; item += gridDim.x) {
-    // Numbers of row tiles: sequence b has those from cu[b] / rows + b on, which is room for all its tiles, so that a tile's
-    // sequence is found without the others' sum.  The last rows of a sequence, which take longest, come first.
-    const int number = p.slots - 1 - item / p.per_slot, at = item % p.per_slot;
-    int lo = 0, hi = p.batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (__ldg(p.cu_seqlens + mid) / rows + mid <= number) lo = mid; else hi = mid;
-    }
-    w.begin = __ldg(p.cu_seqlens + lo);
-    const int end = __ldg(p.cu_seqlens + lo + 1);
-    if (w.begin < 0 || end < w.begin || end > p.tokens) {
-      if (p.index_word) *p.index_word = kBadIndex;
-      continue;
-    }
-    w.len = end - w.begin;
-    const int row = (number - w.begin / rows - lo) * rows;
-    if (row < 0 || row >= w.len) continue;
-    w.row[0] = row;
-    w.row[1] = p.pair_heads ? row : row + kTile;
-    w.head[0] = p.pair_heads ? 2 * at : at;
-    w.head[1] = p.pair_heads ? 2 * at + 1 : at;
-    w.kv = w.head[0] / p.group;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) w.steps[i] = w.row[i] < w.len ? w.row[i] / kTile + 1 : 0;
-    return true;
+// The items of a block, in turn, found by a warp.  With up to 256 sequences the tiles of rows are taken by how many keys they
+// have, longest first, and dealt to the blocks back and forth, so that all blocks have about as much to do (one prompt of
+// 2048 tokens and 32 heads: 74 us dealt in one direction, in which case a third of the SMs' time was idle).  With more, in
+// the order of the batch.
+struct Planner {
+  const PrefillParams& p;
+  int lane, rows, round = 0;
+  int tiles[kSortedBatch / 32];            // of sequences lane, lane + 32, ...
+  int total;                               // tiles of rows in all (sorted), numbers for them (not sorted)
+  int level;                               // tiles with this many in front of them in their sequence are in turn
+
+  __device__ __forceinline__ bool sequence(int b, int& begin, int& len) const {
+    begin = __ldg(p.cu_seqlens + b);
+    const int end = __ldg(p.cu_seqlens + b + 1);
+    const bool good = begin >= 0 && end >= begin && end <= p.tokens;
+    if (!good && p.index_word) *p.index_word = kBadIndex;
+    len = good ? end - begin : 0;
+    return good;
   }
-  return false;
-}
+  __device__ __forceinline__ int beyond(int l) const {        // tiles with at least l in front of them
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < kSortedBatch / 32; ++k) n += max(0, tiles[k] - l);
+    return __reduce_add_sync(0xffffffffu, n);
+  }
+  __device__ __forceinline__ Planner(const PrefillParams& params, int lane_) : p(params), lane(lane_), rows(params.pair_heads ? kTile : 2 * kTile) {
+    total = p.slots;
+    level = 0;
+    if (p.batch > kSortedBatch) return;
+    int most = 0;
+#pragma unroll
+    for (int k = 0; k < kSortedBatch / 32; ++k) {
+      int begin, len = 0;
+      if (k * 32 + lane < p.batch) sequence(k * 32 + lane, begin, len);
+      tiles[k] = (len + rows - 1) / rows;
+      most = max(most, tiles[k]);
+    }
+    level = max(0, __reduce_max_sync(0xffffffffu, most) - 1);
+    total = beyond(0);
+  }
+  // (the whole warp)
+  __device__ __forceinline__ bool next(Work& w) {
+    for (;; ++round) {
+      const int item = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      // (a round's items are all beyond those of the round before)
+      if (item >= total * p.per_slot) return false;
+      const int rank = item / p.per_slot, at = item - rank * p.per_slot;
+      int b, row;
+      if (p.batch <= kSortedBatch) {
+        int lo = 0;                          // the largest level <= the present one with beyond(level) > rank
+        while (lo < level) {
+          const int mid = (lo + level + 1) / 2;
+          if (beyond(mid) > rank) lo = mid; else level = mid - 1;
+        }
+        int index = rank - beyond(level + 1);
+        b = 0;
+#pragma unroll
+        for (int k = 0; k < kSortedBatch / 32; ++k) {
+          const uint32_t there = __ballot_sync(0xffffffffu, tiles[k] > level);
+          const bool me = tiles[k] > level && __popc(there & ((1u << lane) - 1)) == index;
+          const uint32_t who = __ballot_sync(0xffffffffu, me);
+          if (who) b = k * 32 + __ffs(who) - 1;
+          index -= __popc(there);
+        }
+        row = level * rows;
+      } else {
+        // Numbers of row tiles: sequence b has those from cu[b] / rows + b on, which is room for all its tiles, so that a
+        // tile's sequence is found without the others' sum.
+        const int number = p.slots - 1 - rank;
+        int lo = 0, hi = p.batch;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (__ldg(p.cu_seqlens + mid) / rows + mid <= number) lo = mid; else hi = mid;
+        }
+        b = lo;
+        row = (number - __ldg(p.cu_seqlens + b) / rows - b) * rows;
+      }
+      if (!sequence(b, w.begin, w.len) || row < 0 || row >= w.len) continue;
+      ++round;
+      w.row[0] = row;
+      w.row[1] = p.pair_heads ? row : row + kTile;
+      w.head[0] = p.pair_heads ? 2 * at : at;
+      w.head[1] = p.pair_heads ? 2 * at + 1 : at;
+      w.kv = w.head[0] / p.group;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) w.steps[i] = w.row[i] < w.len ? w.row[i] / kTile + 1 : 0;
+      return true;
+    }
+  }
+};
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -170,12 +285,15 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (2 + C::kStages) * C::kTileBytes);
   const uint32_t q_tile = smem_u32(smem), ring = q_tile + 2 * C::kTileBytes;
   const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * C::kStages, q_full = kv_empty + 8 * C::kStages,
-                 q_empty = q_full + 16, s_full = q_empty + 16, p_ready = s_full + 16, o_done = p_ready + 16, scanned = o_done + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 12);
+                 q_empty = q_full + 16, s_full = q_empty + 16, p_ready = s_full + 16 /* [tile][half of the keys] */,
+                 o_done = p_ready + 32, scanned = o_done + 16, work_full = scanned + 16, work_empty = work_full + 8 * kAhead;
+  constexpr int kBars = 2 * C::kStages + 14 + 2 * kAhead;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // [tile][item's parity]: the last product of the tile's item is not the MMA's
   volatile int* odd_values = reinterpret_cast<volatile int*>(tmem_slot + 2);
-  static_assert(8 * (2 * C::kStages + 12) + 24 <= C::kBarBytes, "");
+  Work* works = reinterpret_cast<Work*>(tmem_slot + 6);
+  static_assert(8 * kBars + 24 + kAhead * sizeof(Work) <= C::kBarBytes, "");
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -187,10 +305,15 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       mbar_init(q_full + 8 * i, 1);
       mbar_init(q_empty + 8 * i, 1);
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_ready + 8 * i, 4);
+      mbar_init(p_ready + 16 * i, 4);
+      mbar_init(p_ready + 16 * i + 8, 4);
       mbar_init(o_done + 8 * i, 1);
       mbar_init(scanned + 8 * i, 4);
       odd_values[2 * i] = odd_values[2 * i + 1] = 0;
+    }
+    for (int a = 0; a < kAhead; ++a) {
+      mbar_init(work_full + 8 * a, 1);
+      mbar_init(work_empty + 8 * a, 10);       // the copying and the multiplying thread, eight warps
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -209,11 +332,20 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   chain_wait();
   chain_release();
 
-  int item = blockIdx.x;
   Work w;
+  int taken = 0;                               // items this role has taken
   // (each side's code hangs below its own setmaxnreg, or the compiler holds all of it to the smaller number)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    // the next item, for a role of one thread
+    auto take = [&](Work& x) {
+      const int a = taken % kAhead;
+      if (!mbar_wait(work_full + 8 * a, (taken / kAhead) & 1, abort_flag)) return false;
+      x = works[a];
+      mbar_arrive(work_empty + 8 * a);
+      ++taken;
+      return x.steps[0] != 0;
+    };
     if (warp == 0 && elect_one()) {
       int load = 0;                            // copies of keys and values so far
       uint32_t q_phase[2] = {1, 1};
@@ -233,7 +365,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         ++load;
         return true;
       };
-      for (; ok && next_work(p, item, w); item += gridDim.x) {
+      while (ok && take(w)) {
         const int steps = max(w.steps[0], w.steps[1]);
         uint32_t dst, bar;
 #pragma unroll
@@ -262,9 +394,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       constexpr uint32_t kFormats = kIdescDFormatF32 | (__is_same(T, __half) ? 0u : (1u << 7) | (1u << 10));
       constexpr uint32_t kIdescQK = umma_idesc(kFormats, kTile, kTile);
       constexpr uint32_t kIdescPV = umma_idesc(kFormats, kTile, DP) | (1u << 16);      // B's rows in memory are K
-      int load = 0;
+      int load = 0;                            // the copy of the item's first keys
       uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, parity[2] = {0, 0};
-      bool ok = true;
       auto full = [&](int n) { return mbar_wait(kv_full + 8 * (n % C::kStages), (n / C::kStages) & 1, abort_flag); };
       auto scores = [&](int i, int n) {        // S_i = Q_i K^T with the keys of copy n
         const uint64_t a = umma_desc_k_sw128(q_tile + i * C::kTileBytes);
@@ -276,48 +407,81 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         umma_commit(s_full + 8 * i);
       };
-      for (; ok && next_work(p, item, w); item += gridDim.x) {
-        const int steps = max(w.steps[0], w.steps[1]);
-        if (!full(load)) break;
+      // The first scores of an item follow the last product of the one before, tile by tile: the ring's order is that of the
+      // keys' and values' first use by either tile, and it has room for the two or three copies that a tile may be ahead.
+      auto first_scores = [&](int i, int steps, int n) {
+        if (!mbar_wait(q_full + 8 * i, q_phase[i], abort_flag) || !full(n)) return false;
+        q_phase[i] ^= 1;
+        tcgen05_fence_after();
+        scores(i, n);
+        if (steps == 1) umma_commit(q_empty + 8 * i);
+        return true;
+      };
+      bool more = take(w), ok = true;
+      if (more) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (!w.steps[i]) continue;
-          if (!mbar_wait(q_full + 8 * i, q_phase[i], abort_flag)) { ok = false; break; }
-          q_phase[i] ^= 1;
-          tcgen05_fence_after();
-          scores(i, load);
-          if (w.steps[i] == 1) umma_commit(q_empty + 8 * i);
-        }
+        for (int i = 0; i < 2; ++i) ok = ok && (!w.steps[i] || first_scores(i, w.steps[i], load));
         umma_commit(kv_empty + 8 * (load % C::kStages));
+      }
+      while (ok && more) {
+        Work then;
+        more = take(then);
+        const int steps = max(w.steps[0], w.steps[1]), next_load = load + 2 * steps;
         for (int j = 0; ok && j < steps; ++j) {
           const int nv = load + 2 * j + 1, nk = nv + 1;       // the copies of this step's values and the next one's keys
           if (!full(nv)) { ok = false; break; }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (j >= w.steps[i]) continue;
-            if (!mbar_wait(p_ready + 8 * i, p_phase[i], abort_flag)) { ok = false; break; }
-            p_phase[i] ^= 1;
-            tcgen05_fence_after();
-            if (j + 1 < w.steps[i] || !odd_values[2 * i + parity[i]]) {
-              const uint64_t b = umma_desc_rows_sw128(ring + (nv % C::kStages) * C::kTileBytes);
+            const bool last = j + 1 == w.steps[i];
+            const uint64_t b = umma_desc_rows_sw128(ring + (nv % C::kStages) * C::kTileBytes);
+            bool multiply = true;
 #pragma unroll
-              for (int k = 0; k < kTile / 16; ++k)
-                umma_ts(tmem + 2 * kTile + i * DP, tmem + i * kTile + k * 8, b + k * ((16 * 128) >> 4), kIdescPV, j != 0 || k != 0);
-            }
-            umma_commit(o_done + 8 * i);
-            if (j + 1 == w.steps[i]) {
-              parity[i] ^= 1;
-            } else {
-              if (!full(nk)) { ok = false; break; }
+            for (int half = 0; half < 2; ++half) {            // the weights come in halves of the keys
+              if (!mbar_wait(p_ready + 16 * i + 8 * half, p_phase[i], abort_flag)) { ok = false; break; }
               tcgen05_fence_after();
+              if (half == 0 && last) multiply = !odd_values[2 * i + parity[i]];
+              if (multiply) {
+#pragma unroll
+                for (int k = 4 * half; k < 4 * half + 4; ++k)
+                  umma_ts(tmem + 2 * kTile + i * DP, tmem + i * kTile + k * 8, b + k * ((16 * 128) >> 4), kIdescPV, j != 0 || k != 0);
+              }
+            }
+            if (!ok) break;
+            p_phase[i] ^= 1;
+            umma_commit(o_done + 8 * i);
+            if (!last) {
+              if (!full(nk)) { ok = false; break; }
               scores(i, nk);
               if (j + 2 == w.steps[i]) umma_commit(q_empty + 8 * i);
+            } else {
+              parity[i] ^= 1;
+              if (more && then.steps[i] && !first_scores(i, then.steps[i], next_load)) { ok = false; break; }
             }
           }
           umma_commit(kv_empty + 8 * (nv % C::kStages));
           if (j + 1 < steps) umma_commit(kv_empty + 8 * (nk % C::kStages));
         }
-        load += 2 * steps;
+        if (!ok || !more) break;
+        if (!w.steps[1] && then.steps[1] && !first_scores(1, then.steps[1], next_load)) break;
+        umma_commit(kv_empty + 8 * (next_load % C::kStages));
+        w = then;
+        load = next_load;
+      }
+    }
+    if (warp == 2) {
+      Planner plan(p, lane);
+      for (bool more = true; more; ++taken) {
+        w.steps[0] = 0;
+        more = plan.next(w);
+        if (!more) w.steps[0] = 0;
+        const int a = taken % kAhead;
+        if (!__all_sync(0xffffffffu, mbar_wait(work_empty + 8 * a, ((taken / kAhead) & 1) ^ 1, abort_flag))) break;
+        if (lane == 0) {
+          works[a] = w;
+          mbar_arrive(work_full + 8 * a);
+        }
+        __syncwarp();
       }
     }
   } else {
@@ -329,11 +493,21 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     uint32_t s_phase = 0, o_phase = 0, scan_phase = 0;         // o_phase: of the next product to complete
     int load = 0;
     bool ok = true;
+    const F2 scale2 = f2(p.negative ? -p.scale_log2 : p.scale_log2, p.negative ? -p.scale_log2 : p.scale_log2);
     auto wait_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
-    for (; ok && next_work(p, item, w); item += gridDim.x) {
-      const int steps = i ? w.steps[1] : w.steps[0], row_begin = i ? w.row[1] : w.row[0], head = i ? w.head[1] : w.head[0];
+    while (ok) {
+      const int slot = taken % kAhead;
+      if (!wait_all(work_full + 8 * slot, (taken / kAhead) & 1)) break;
+      const Work& next = works[slot];
+      const int steps = next.steps[i], row_begin = next.row[i], head = next.head[i], seq_begin = next.begin, len = next.len;
+      const int item_steps = max(next.steps[0], next.steps[1]);
+      const bool end = next.steps[0] == 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(work_empty + 8 * slot);
+      ++taken;
+      if (end) break;
       const int first_load = load;
-      load += 2 * max(w.steps[0], w.steps[1]);
+      load += 2 * item_steps;
       if (!steps) continue;
       float m = kNegInf, sum = 0.0f;
       for (int j = 0; j < steps; ++j) {
@@ -346,72 +520,94 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_tmem + 32 * c, s[c]);
         tmem_ld_wait();
         auto value = [&](int c) -> uint32_t& { return s[c >> 5][c & 31]; };
+        if (last) {
+          const uint32_t nothing = __float_as_uint(p.negative ? -kNegInf : kNegInf);
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) value(c) = c <= row ? value(c) : nothing;
+        }
+        if (p.negative) {                      // the largest product is that of the smallest score
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) value(c) ^= 0x80000000u;
+        }
+        // A NaN anywhere makes the maximum NaN, and with it the whole row; so does a score of plus infinity.
+        float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+        for (int c = 0; c < kTile; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(value(c + e)), __uint_as_float(value(c + e + 4)));
+        const float now = max3(m, max3(top[0], top[1], top[2]) * p.scale_log2, top[3] * p.scale_log2);
         if (p.negative) {
 #pragma unroll
           for (int c = 0; c < kTile; ++c) value(c) ^= 0x80000000u;
         }
-        if (last) {
+        // (number j + 1 is the product of this tile that is the next to complete)
+        if (__any_sync(0xffffffffu, !(now <= m + kGrowth)) || j == 0) {
+          const float grown = now == -kNegInf ? __uint_as_float(0x7fffffffu) : now;
+          if (j > 0) {
+            if (!wait_all(o_done + 8 * i, o_phase ^ 1)) { ok = false; break; }    // product j
+            tcgen05_fence_after();
+            const float keep = grown == kNegInf ? 1.0f : exp2_fast(m - grown);
+            sum *= keep;
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32(o_tmem + 32 * c, o);
+              tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < kTile; ++c) value(c) = c <= row ? value(c) : __float_as_uint(kNegInf);
-        }
-        float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-#pragma unroll
-        for (int c = 0; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(value(c)));
-        const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2);
-        // products of this tile that are complete: j (the next to complete is number j + 1)
-        if (j == 0) {
-          m = now;
-        } else if (__any_sync(0xffffffffu, now > m + kGrowth)) {
-          if (!wait_all(o_done + 8 * i, o_phase ^ 1)) { ok = false; break; }      // product j
-          tcgen05_fence_after();
-          const float keep = now == kNegInf ? 1.0f : exp2_fast(m - now);
-          sum *= keep;
-          m = now;
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(o_tmem + 32 * c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-            tmem_st_32x32(o_tmem + 32 * c, o);
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tmem_st_32x32(o_tmem + 32 * c, o);
+            }
           }
+          m = grown;
         }
         o_phase ^= 1;
         const float ref = m == kNegInf ? 0.0f : m;
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const F2 minus_ref = f2(-ref, -ref);
+        F2 part[2] = {0, 0};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t packed[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int c = h * 64 + 2 * e;
-            const float a = exp2_fast(fmaf(__uint_as_float(value(c)), p.scale_log2, -ref));
-            const float b = exp2_fast(fmaf(__uint_as_float(value(c + 1)), p.scale_log2, -ref));
-            part[e & 1] += a;
-            part[2 + (e & 1)] += b;
+            const F2 x = fma2(f2(__uint_as_float(value(c)), __uint_as_float(value(c + 1))), scale2, minus_ref);
+            float a, b;
+            if (e % kMultipliedEvery == kMultipliedEvery - 1) {
+              exp2_pair(x, a, b);
+            } else {
+              split(x, a, b);
+              a = exp2_fast(a);
+              b = exp2_fast(b);
+            }
+            part[e & 1] = add2(part[e & 1], f2(a, b));
             packed[e] = pack2<T>(a, b);
           }
           tmem_st_32x32(s_tmem + 32 * h, packed);
+          if (h == 0 && !last) {               // the product with the first half of the keys may begin
+            tmem_st_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready + 16 * i);
+          }
         }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        float part_sum[2];
+        split(add2(part[0], part[1]), part_sum[0], part_sum[1]);
+        sum += part_sum[0] + part_sum[1];
         if (last) {
           // ---- V's rows behind the sequence's end, and values that are not finite
-          const int n = first_load + 2 * j + 1, valid = w.len - j * kTile;
+          const int n = first_load + 2 * j + 1, valid = len - j * kTile;
           if (!wait_all(kv_full + 8 * (n % C::kStages), (n / C::kStages) & 1)) { ok = false; break; }
           const uint32_t tile_v = ring + (n % C::kStages) * C::kTileBytes;
-          bool odd = false;
-#pragma unroll
-          for (int b = 0; b < C::kBoxes; ++b)
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const int r = c * 16 + quarter * 4 + (lane >> 3);           // 16 rows of eight pieces
-              const uint32_t at = tile_v + b * kTile * 128 + r * 128 + (lane & 7) * 16;
-              if (r < valid) odd = odd || any_not_finite<T>(lds16(at));
-              else asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0u) : "memory");
-            }
+          uint32_t zeros = 0;
+#pragma unroll 2
+          for (int c = 0; c < 8 * C::kBoxes; ++c) {
+            const int r = (c & 7) * 16 + quarter * 4 + (lane >> 3);       // 16 rows of eight pieces
+            const uint32_t at = tile_v + (c >> 3) * kTile * 128 + r * 128 + (lane & 7) * 16;
+            if (r < valid) zeros = add_zeros<T>(zeros, lds16(at));
+            else asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0u) : "memory");
+          }
           if (valid < kTile) fence_proxy_async_smem();
-          if (__any_sync(0xffffffffu, odd) && lane == 0) odd_values[2 * i + scan_phase] = 1;
+          if (__any_sync(0xffffffffu, (zeros & 0x7fff7fffu) != 0) && lane == 0) odd_values[2 * i + scan_phase] = 1;
           // (whoever read the other one, for the item before, has done so: that item's last product is complete)
           if (quarter == 0 && lane == 0) odd_values[2 * i + (scan_phase ^ 1)] = 0;
           mbar_arrive_warp(scanned + 8 * i, lane);
@@ -424,6 +620,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
               if (!wait_all(o_done + 8 * i, o_phase)) { ok = false; break; }      // product j, of the tile before
               tcgen05_fence_after();
             }
+#pragma unroll 1
             for (int d0 = 0; d0 < DP; d0 += 32) {
               uint32_t o[32];
               if (j > 0) {
@@ -433,6 +630,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = 0u;
               }
+#pragma unroll 1
               for (int c = 0; c < kTile; c += 2) {
                 const float2 pair = unpack2<T>(tmem_ld_column(s_tmem + c / 2));
 #pragma unroll
@@ -460,7 +658,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tmem_st_wait();
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready + 8 * i);
+        if (lane == 0) {
+          if (last) mbar_arrive(p_ready + 16 * i);
+          mbar_arrive(p_ready + 16 * i + 8);
+        }
       }
       if (!ok) break;
       // ---- the row's result
@@ -468,13 +669,13 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       tcgen05_fence_after();
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       const int at = row_begin + row;
-      char* dst = p.out + ((static_cast<long long>(w.begin) + at) * p.q_heads + head) * p.dim * 2;
-#pragma unroll
+      char* dst = p.out + ((static_cast<long long>(seq_begin) + at) * p.q_heads + head) * p.dim * 2;
+#pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         uint32_t o[32];
         tmem_ld_32x32(o_tmem + 32 * c, o);
         tmem_ld_wait();
-        if (at < w.len) {
+        if (at < len) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint32_t word[4];
