@@ -34,7 +34,6 @@ constexpr int kWarps = 12, kThreads = 32 * kWarps;
 constexpr int kFewRegisters = 56, kManyRegisters = 224;
 constexpr int kTmemCols = 512;
 constexpr float kGrowth = 8.0f;                // log2 of how far weights may exceed 1
-constexpr int kMultipliedEvery = 4;            // one pair of exponentials in so many by multiplications
 constexpr int kAhead = 4;                      // items that the planning warp is ahead
 constexpr int kSortedBatch = 256;              // sequences whose tiles are taken longest first
 
@@ -61,23 +60,25 @@ struct PrefillParams {
   int pair_heads;                              // the block's two tiles: 1 two heads, 0 two tiles of a head
   int slots, per_slot;                         // numbers of row tiles, and the items of each
   float scale_log2;                            // |scale| log2 e
-  int negative;                                // scale < 0
+  uint32_t negate;                             // scale < 0: the bit of the products' descriptor that negates Q
   MapOrder q_order, k_order, v_order;
 };
 
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Products with a descriptor's low word and the high word that all of a layout share; ACC: added to what is there.
+template <bool ACC>
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t a_hi, uint32_t b, uint32_t b_hi, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .b64 a, b;\n\t.reg .pred p;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(a_hi), "r"(b), "r"(b_hi), "r"(idesc), "n"(ACC ? 1 : 0) : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .b64 b;\n\t.reg .pred p;\n\tmov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -121,7 +122,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// Pairs of fp32 values in one instruction.
+// Pairs of fp32 values in one instruction.  (volatile: in the order they are written in, which exp2_batch is about)
 using F2 = unsigned long long;
 __device__ __forceinline__ F2 f2(float a, float b) {
   F2 r;
@@ -131,37 +132,73 @@ __device__ __forceinline__ F2 f2(float a, float b) {
 __device__ __forceinline__ void split(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ float exp2_ordered(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-// 2^x of a pair by multiplications: x = n + f with n the nearest integer, 2^f by a polynomial of degree 5 (minimax on
-// [-1/2, 1/2], found by exchange; relative error 2^-23.6), n added to the exponent.  x is at most 2^7; below -127 it counts
-// as -127, which gives 0.  The exponential unit takes 16 values a clock and SM, the tensor cores a product of 128 x 128 x 128
-// in the time of 8192: a share of them taken here shortens a tile's turn.  (A NaN does not come through: see the maximum.)
-__device__ __forceinline__ void exp2_pair(F2 x, float& a, float& b) {
+// Weights 2^(s scale - ref) of 16 scores, their sum added to `sum` and the weights rounded to eight words.  Two of the eight
+// pairs are computed by multiplications while the exponential unit has the others: x = n + f with n the nearest integer, 2^f
+// by a polynomial of degree 5 (minimax on [-1/2, 1/2], found by exchange; relative error 2^-23.6), n added to the exponent.
+// x is at most about 2^7; below -127 it counts as -127, which gives 0.  (A NaN does not come through there: see the maximum.)
+// The unit takes 16 values a clock and SM; with one warp on a scheduler 128 scores take 984 clocks in this order and 1650
+// as the compiler orders a plain loop, with two 1704 together and 2100 without the multiplications.
+// between(m), m = 0..6: what else can be done meanwhile.
+template <typename T, typename F>
+__device__ __forceinline__ void exp2_batch(const uint32_t* s, F2 scale, F2 minus_ref, F2& sum, uint32_t* packed, F between) {
   constexpr float kMagic = 12582912.0f;        // 1.5 * 2^23: added, the sum's low bits are the nearest integer
-  float x0, x1;
-  split(x, x0, x1);
-  x = f2(fmaxf(x0, -127.0f), fmaxf(x1, -127.0f));
-  const F2 t = add2(x, f2(kMagic, kMagic));
-  const F2 f = add2(x, fma2(t, f2(-1.0f, -1.0f), f2(kMagic, kMagic)));
-  F2 r = f2(1.3276472454890609e-3f, 1.3276472454890609e-3f);
-  r = fma2(r, f, f2(9.675540961325169e-3f, 9.675540961325169e-3f));
-  r = fma2(r, f, f2(5.550713092088699e-2f, 5.550713092088699e-2f));
-  r = fma2(r, f, f2(0.24022120237350464f, 0.24022120237350464f));
-  r = fma2(r, f, f2(0.6931469440460205f, 0.6931469440460205f));
-  r = fma2(r, f, f2(1.0000001192092896f, 1.0000001192092896f));
-  float t0, t1;
-  split(t, t0, t1);
-  split(r, a, b);
-  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
-  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
+  constexpr float kC[6] = {1.3276472454890609e-3f, 9.675540961325169e-3f, 5.550713092088699e-2f,
+                           0.24022120237350464f, 0.6931469440460205f, 1.0000001192092896f};
+  F2 x[8], t[2], f[2], r[2];
+  float v[16];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = fma2(f2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale, minus_ref);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float a, b;
+    split(x[6 + e], a, b);
+    x[6 + e] = f2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
+    t[e] = add2(x[6 + e], f2(kMagic, kMagic));
+  }
+#pragma unroll
+  for (int m = 0; m < 7; ++m) {
+    if (m < 6) {
+      float a, b;
+      split(x[m], a, b);
+      v[2 * m] = exp2_ordered(a);
+      v[2 * m + 1] = exp2_ordered(b);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (m == 0) f[e] = fma2(t[e], f2(-1.0f, -1.0f), f2(kMagic, kMagic));
+      if (m == 1) f[e] = add2(x[6 + e], f[e]);
+      if (m == 2) r[e] = fma2(f2(kC[0], kC[0]), f[e], f2(kC[1], kC[1]));
+      if (m > 2) r[e] = fma2(r[e], f[e], f2(kC[m - 1], kC[m - 1]));
+    }
+    between(m);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float a, b, t0, t1;
+    split(r[e], a, b);
+    split(t[e], t0, t1);
+    v[12 + 2 * e] = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
+    v[13 + 2 * e] = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    sum = add2(sum, f2(v[2 * e], v[2 * e + 1]));
+    packed[e] = pack2<T>(v[2 * e], v[2 * e + 1]);
+  }
 }
 
 // Descriptor of V as the B operand [dims x keys] whose rows in memory are keys (128 bytes of 64 dims, 128-byte swizzle):
@@ -328,7 +365,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   chain_wait();
   chain_release();
 
@@ -392,81 +429,114 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     }
     if (warp == 1 && elect_one()) {
       constexpr uint32_t kFormats = kIdescDFormatF32 | (__is_same(T, __half) ? 0u : (1u << 7) | (1u << 10));
-      constexpr uint32_t kIdescQK = umma_idesc(kFormats, kTile, kTile);
+      const uint32_t idesc_qk = umma_idesc(kFormats, kTile, kTile) | p.negate;
       constexpr uint32_t kIdescPV = umma_idesc(kFormats, kTile, DP) | (1u << 16);      // B's rows in memory are K
-      int load = 0;                            // the copy of the item's first keys
+      const uint64_t k_desc = umma_desc_k_sw128(ring), v_desc = umma_desc_rows_sw128(ring);
+      const uint32_t k_lo = static_cast<uint32_t>(k_desc), k_hi = static_cast<uint32_t>(k_desc >> 32);
+      const uint32_t v_lo = static_cast<uint32_t>(v_desc), v_hi = static_cast<uint32_t>(v_desc >> 32);
+      const uint32_t q_lo = static_cast<uint32_t>(umma_desc_k_sw128(q_tile));
+      constexpr uint32_t kTileStep = C::kTileBytes >> 4;
+      auto wait = [&](uint32_t bar, uint32_t phase) { return mbar_wait(bar, phase, abort_flag); };
+      struct Slot {                            // of the ring, in the order of the copies
+        uint32_t at = 0, phase = 0;
+        __device__ __forceinline__ void step(int n) {
+          at += n;
+          if (at >= C::kStages) { at -= C::kStages; phase ^= 1; }
+        }
+      };
       uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, parity[2] = {0, 0};
-      auto full = [&](int n) { return mbar_wait(kv_full + 8 * (n % C::kStages), (n / C::kStages) & 1, abort_flag); };
-      auto scores = [&](int i, int n) {        // S_i = Q_i K^T with the keys of copy n
-        const uint64_t a = umma_desc_k_sw128(q_tile + i * C::kTileBytes);
-        const uint64_t b = umma_desc_k_sw128(ring + (n % C::kStages) * C::kTileBytes);
+      auto full = [&](const Slot& s) { return wait(kv_full + 8 * s.at, s.phase); };
+      auto scores = [&](int i, const Slot& s) {               // S_i = Q_i K^T
+        const uint32_t a = q_lo + i * kTileStep, b = k_lo + s.at * kTileStep;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t at = (k >> 2) * ((kTile * 128) >> 4) + 2 * (k & 3);
-          umma_ss(tmem + i * kTile, a + at, b + at, kIdescQK, k != 0);
+          if (k == 0) umma_ss<false>(tmem + i * kTile, a + at, k_hi, b + at, k_hi, idesc_qk);
+          else umma_ss<true>(tmem + i * kTile, a + at, k_hi, b + at, k_hi, idesc_qk);
         }
         umma_commit(s_full + 8 * i);
       };
+      auto release = [&](const Slot& s) { umma_commit(kv_empty + 8 * s.at); };
+      int steps[2], then[2];
+      auto take_steps = [&](int (&n)[2]) {     // of the next item
+        const int a = taken % kAhead;
+        if (!wait(work_full + 8 * a, (taken / kAhead) & 1)) return false;
+        n[0] = works[a].steps[0];
+        n[1] = works[a].steps[1];
+        mbar_arrive(work_empty + 8 * a);
+        ++taken;
+        return n[0] != 0;
+      };
       // The first scores of an item follow the last product of the one before, tile by tile: the ring's order is that of the
       // keys' and values' first use by either tile, and it has room for the two or three copies that a tile may be ahead.
-      auto first_scores = [&](int i, int steps, int n) {
-        if (!mbar_wait(q_full + 8 * i, q_phase[i], abort_flag) || !full(n)) return false;
+      auto first_scores = [&](int i, int n, const Slot& s) {
+        if (!wait(q_full + 8 * i, q_phase[i]) || !full(s)) return false;
         q_phase[i] ^= 1;
-        tcgen05_fence_after();
-        scores(i, n);
-        if (steps == 1) umma_commit(q_empty + 8 * i);
+        scores(i, s);
+        if (n == 1) umma_commit(q_empty + 8 * i);
         return true;
       };
-      bool more = take(w), ok = true;
+      Slot first;                              // the item's first keys
+      bool more = take_steps(steps), ok = true;
       if (more) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) ok = ok && (!w.steps[i] || first_scores(i, w.steps[i], load));
-        umma_commit(kv_empty + 8 * (load % C::kStages));
+        for (int i = 0; i < 2; ++i) ok = ok && (!steps[i] || first_scores(i, steps[i], first));
+        release(first);
       }
       while (ok && more) {
-        Work then;
-        more = take(then);
-        const int steps = max(w.steps[0], w.steps[1]), next_load = load + 2 * steps;
-        for (int j = 0; ok && j < steps; ++j) {
-          const int nv = load + 2 * j + 1, nk = nv + 1;       // the copies of this step's values and the next one's keys
-          if (!full(nv)) { ok = false; break; }
+        more = take_steps(then);
+        const int most = max(steps[0], steps[1]);
+        Slot v = first, k = first, last_k;     // this step's values and the next one's keys, or the next item's
+        v.step(1);
+        k.step(2);
+        for (int j = 0; ok && j < most; ++j) {
+          if (!full(v)) { ok = false; break; }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            if (j >= w.steps[i]) continue;
-            const bool last = j + 1 == w.steps[i];
-            const uint64_t b = umma_desc_rows_sw128(ring + (nv % C::kStages) * C::kTileBytes);
+            if (j >= steps[i]) continue;
+            const bool last = j + 1 == steps[i];
             bool multiply = true;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {            // the weights come in halves of the keys
-              if (!mbar_wait(p_ready + 16 * i + 8 * half, p_phase[i], abort_flag)) { ok = false; break; }
+              if (!wait(p_ready + 16 * i + 8 * half, p_phase[i])) { ok = false; break; }
               tcgen05_fence_after();
-              if (half == 0 && last) multiply = !odd_values[2 * i + parity[i]];
+              if (half == 0 && last) multiply = odd_values[2 * i + parity[i]] == 0;
               if (multiply) {
+                const uint32_t b = v_lo + v.at * kTileStep;
 #pragma unroll
                 for (int k = 4 * half; k < 4 * half + 4; ++k)
-                  umma_ts(tmem + 2 * kTile + i * DP, tmem + i * kTile + k * 8, b + k * ((16 * 128) >> 4), kIdescPV, j != 0 || k != 0);
+                  umma_ts(tmem + 2 * kTile + i * DP, tmem + i * kTile + k * 8, b + k * ((16 * 128) >> 4), v_hi, kIdescPV, k != 0 ? 1u : j != 0);
               }
             }
             if (!ok) break;
             p_phase[i] ^= 1;
             umma_commit(o_done + 8 * i);
             if (!last) {
-              if (!full(nk)) { ok = false; break; }
-              scores(i, nk);
-              if (j + 2 == w.steps[i]) umma_commit(q_empty + 8 * i);
+              if (!full(k)) { ok = false; break; }
+              scores(i, k);
+              if (j + 2 == steps[i]) umma_commit(q_empty + 8 * i);
             } else {
               parity[i] ^= 1;
-              if (more && then.steps[i] && !first_scores(i, then.steps[i], next_load)) { ok = false; break; }
+              if (more && then[i]) {
+                Slot next = k;                 // the next item's first keys: two copies on if tile 1 has one step more
+                if (j + 1 < most) next.step(2);
+                if (!first_scores(i, then[i], next)) { ok = false; break; }
+              }
             }
           }
-          umma_commit(kv_empty + 8 * (nv % C::kStages));
-          if (j + 1 < steps) umma_commit(kv_empty + 8 * (nk % C::kStages));
+          if (!ok) break;
+          release(v);
+          if (j + 1 < most) release(k);
+          last_k = k;
+          v.step(2);
+          k.step(2);
         }
         if (!ok || !more) break;
-        if (!w.steps[1] && then.steps[1] && !first_scores(1, then.steps[1], next_load)) break;
-        umma_commit(kv_empty + 8 * (next_load % C::kStages));
-        w = then;
-        load = next_load;
+        first = last_k;
+        if (!steps[1] && then[1] && !first_scores(1, then[1], first)) break;
+        release(first);
+        steps[0] = then[0];
+        steps[1] = then[1];
       }
     }
     if (warp == 2) {
@@ -493,7 +563,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     uint32_t s_phase = 0, o_phase = 0, scan_phase = 0;         // o_phase: of the next product to complete
     int load = 0;
     bool ok = true;
-    const F2 scale2 = f2(p.negative ? -p.scale_log2 : p.scale_log2, p.negative ? -p.scale_log2 : p.scale_log2);
+    const F2 scale2 = f2(p.scale_log2, p.scale_log2);
     auto wait_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
     while (ok) {
       const int slot = taken % kAhead;
@@ -521,77 +591,68 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tmem_ld_wait();
         auto value = [&](int c) -> uint32_t& { return s[c >> 5][c & 31]; };
         if (last) {
-          const uint32_t nothing = __float_as_uint(p.negative ? -kNegInf : kNegInf);
 #pragma unroll
-          for (int c = 0; c < kTile; ++c) value(c) = c <= row ? value(c) : nothing;
+          for (int c = 0; c < kTile; ++c) value(c) = c <= row ? value(c) : __float_as_uint(kNegInf);
         }
-        if (p.negative) {                      // the largest product is that of the smallest score
+        // The weights are taken with the maximum of the steps before (the first step's own at first): it is still good if no
+        // score exceeds it by 8.  The scores' maximum is found beside the first half's exponentials; where it exceeds, the
+        // half is taken once more.  A NaN anywhere makes the maximum NaN, and with it the whole row; so does plus infinity.
+        float top[4];
+        auto look = [&](int c) {
 #pragma unroll
-          for (int c = 0; c < kTile; ++c) value(c) ^= 0x80000000u;
+          for (int e = 0; e < 4; ++e)
+            top[e] = max3(c ? top[e] : __uint_as_float(value(e)), __uint_as_float(value(c + e)), __uint_as_float(value(c + e + 4)));
+        };
+        auto maximum = [&]() { return max3(m, max3(top[0], top[1], top[2]) * p.scale_log2, top[3] * p.scale_log2); };
+        auto usable = [&](float now) { return now == -kNegInf ? __uint_as_float(0x7fffffffu) : now; };
+        if (j == 0) {
+#pragma unroll
+          for (int c = 0; c < kTile; c += 8) look(c);
+          m = usable(maximum());
         }
-        // A NaN anywhere makes the maximum NaN, and with it the whole row; so does a score of plus infinity.
-        float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+        F2 part, minus_ref;
+        uint32_t packed[32];
+        for (bool again = j == 0;; again = true) {
+          const float ref = m == kNegInf ? 0.0f : m;
+          minus_ref = f2(-ref, -ref);
+          part = 0;
 #pragma unroll
-        for (int c = 0; c < kTile; c += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(value(c + e)), __uint_as_float(value(c + e + 4)));
-        const float now = max3(m, max3(top[0], top[1], top[2]) * p.scale_log2, top[3] * p.scale_log2);
-        if (p.negative) {
-#pragma unroll
-          for (int c = 0; c < kTile; ++c) value(c) ^= 0x80000000u;
-        }
-        // (number j + 1 is the product of this tile that is the next to complete)
-        if (__any_sync(0xffffffffu, !(now <= m + kGrowth)) || j == 0) {
-          const float grown = now == -kNegInf ? __uint_as_float(0x7fffffffu) : now;
-          if (j > 0) {
-            if (!wait_all(o_done + 8 * i, o_phase ^ 1)) { ok = false; break; }    // product j
-            tcgen05_fence_after();
-            const float keep = grown == kNegInf ? 1.0f : exp2_fast(m - grown);
-            sum *= keep;
-#pragma unroll 1
-            for (int c = 0; c < DP / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld_32x32(o_tmem + 32 * c, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-              tmem_st_32x32(o_tmem + 32 * c, o);
-            }
-          }
+          for (int b = 0; b < 4; ++b)
+            exp2_batch<T>(&value(16 * b), scale2, minus_ref, part, packed + 8 * b, [&](int step) {
+              if (step < 4) look(32 * b + 8 * step);
+            });
+          const float now = maximum();
+          if (again || !__any_sync(0xffffffffu, !(now <= m + kGrowth))) break;
+          // (number j + 1 is the product of this tile that is the next to complete)
+          if (!wait_all(o_done + 8 * i, o_phase ^ 1)) { ok = false; break; }      // product j
+          tcgen05_fence_after();
+          const float grown = usable(now), keep = grown == kNegInf ? 1.0f : exp2_fast(m - grown);
+          sum *= keep;
           m = grown;
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(o_tmem + 32 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+            tmem_st_32x32(o_tmem + 32 * c, o);
+          }
         }
+        if (!ok) break;
         o_phase ^= 1;
-        const float ref = m == kNegInf ? 0.0f : m;
-        const F2 minus_ref = f2(-ref, -ref);
-        F2 part[2] = {0, 0};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t packed[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int c = h * 64 + 2 * e;
-            const F2 x = fma2(f2(__uint_as_float(value(c)), __uint_as_float(value(c + 1))), scale2, minus_ref);
-            float a, b;
-            if (e % kMultipliedEvery == kMultipliedEvery - 1) {
-              exp2_pair(x, a, b);
-            } else {
-              split(x, a, b);
-              a = exp2_fast(a);
-              b = exp2_fast(b);
-            }
-            part[e & 1] = add2(part[e & 1], f2(a, b));
-            packed[e] = pack2<T>(a, b);
-          }
-          tmem_st_32x32(s_tmem + 32 * h, packed);
-          if (h == 0 && !last) {               // the product with the first half of the keys may begin
-            tmem_st_wait();
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready + 16 * i);
-          }
+        tmem_st_32x32(s_tmem, packed);
+        if (!last) {                           // the product with the first half of the keys may begin
+          tmem_st_wait();
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_ready + 16 * i);
         }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) exp2_batch<T>(&value(64 + 16 * b), scale2, minus_ref, part, packed + 8 * b, [](int) {});
+        tmem_st_32x32(s_tmem + 32, packed);
         float part_sum[2];
-        split(add2(part[0], part[1]), part_sum[0], part_sum[1]);
+        split(part, part_sum[0], part_sum[1]);
         sum += part_sum[0] + part_sum[1];
         if (last) {
           // ---- V's rows behind the sequence's end, and values that are not finite
@@ -765,7 +826,7 @@ extern "C" int mp_attention_prefill(int dtype, const mp_head_rows* q, const mp_h
   p.per_slot = p.pair_heads ? Hq / 2 : Hq;
   if (static_cast<long long>(p.slots) * p.per_slot > 0x7fff0000LL) return MP_ERR_UNSUPPORTED;
   p.scale_log2 = fmaxf(fabsf(scale) * attn::kLog2e, 1e-30f);      // masked scores stay minus infinity with a scale of 0 too
-  p.negative = scale < 0.0f;
+  p.negate = scale < 0.0f ? 1u << 13 : 0u;
   CUtensorMap mq, mk, mv;
   if ((rc = head_map(&mq, dtype, qr, T, Hq, D, &p.q_order)) || (rc = head_map(&mk, dtype, kr, T, Hkv, D, &p.k_order)) ||
       (rc = head_map(&mv, dtype, vr, T, Hkv, D, &p.v_order)))
