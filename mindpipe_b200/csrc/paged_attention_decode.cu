@@ -7,12 +7,19 @@
 // of them (mma.sync: at HBM's rate an SM multiplies one 16 x 16 piece of the cache in about 10 clocks, far below what even
 // this path of the tensor cores takes; tcgen05's 128 rows would be 7/8 padding or more).
 //
-// All lengths are known on the device only (a captured launch serves every later step), so the work is cut there: the
-// sequence of (sequence, head) pairs, each in steps of a few keys, is cut evenly over the blocks, two to an SM.  A warp is a
-// stream of its own: it copies its tiles of keys and values to its part of shared memory, several ahead, also across the ends
-// of sequences, and keeps its own maximum, sum and output until the block joins its four warps.  Where a sequence spans
-// blocks they leave (m, sum, o) in the workspace, and the one that arrives last joins them in the blocks' order, so results
-// do not depend on which one that was.
+// All lengths are known on the device only (a captured launch serves every later step), so the work is cut there: the list of
+// (sequence, head) items, each in steps of a few keys, is cut evenly over teams of four warps, two teams to an SM, so that
+// one copies while the other joins.  A warp is a stream of its own: it copies its tiles of keys and values to its part of
+// shared memory (cp.async: a lane's 16 bytes go where ldmatrix finds them without conflicts, and what is not to be read
+// becomes zero; TMA's boxes of 128 bytes a row came at 6.0 TB/s where these come at 6.4), several ahead, also across the
+// ends of sequences, and it keeps its own maximum, sum and output until the team joins at the item's end.  The warps of a team take neighbouring tiles (with a run of tiles for
+// each warp, and no joins but at the run's ends, the cache's rate fell from 6.4 to 5.7 TB/s).  Where an item spans teams they
+// leave (m, sum, o) in the workspace, and the one that arrives last joins them in the teams' order, so results do not depend
+// on which one that was.  Of short sequences, where there are many, a team's warps take an item each, four heads at a time, and
+// need not join (301 sequences of 1 to 700 tokens and five heads: 25 us with four warps to every item).
+//
+// What runs once a launch runs from cold instruction caches, some ten clocks an instruction, and a step's worth of keys is
+// 1.5 us: the code in front of the first tile and at an item's end is kept short.
 #include "attention.cuh"
 
 namespace mp {
@@ -20,24 +27,24 @@ namespace {
 
 using namespace attn;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kTeamWarps = 4, kTeam = 32 * kTeamWarps, kTeams = 2;       // teams of a block
+constexpr int kThreads = kTeam * kTeams;
 constexpr int kStages = 3;
-constexpr int kBlocksPerSm = 2;
-constexpr int kMaxGrid = kSmCount * kBlocksPerSm;
+constexpr int kMaxTeams = kSmCount * kTeams;
 constexpr int kRows = 16;                                     // query heads per tile
 constexpr int kMaxD = 128;
-// Steps that a block takes at least, before more blocks share a short cache.
-constexpr int kMinSteps = 1;
+constexpr int kItemCost = 2;           // what an item costs beside its steps, in steps
+constexpr int kWholeSteps = 4;         // steps up to which an item is not cut: a join of teams takes 2-3 us
+constexpr int kSoloTiles = 8;          // tiles of a sequence up to which a warp takes an item alone, if there are many items
 
-// A block's two parts of sequences that it shares: the one it begins within (0) and the one it ends within (1).
+// A team's two parts of items that it shares: the one it begins within (0) and the one it ends within (1).
 struct PartialTile {
   float m[kRows], sum[kRows];
   float o[kRows][kMaxD];
 };
 constexpr size_t kCounterBytes = 4096;
-static_assert(kMaxGrid * sizeof(int) <= kCounterBytes, "");
-constexpr size_t kWorkspaceBytes = kCounterBytes + sizeof(PartialTile) * kMaxGrid * 2;
+static_assert(kMaxTeams * sizeof(int) <= kCounterBytes, "");
+constexpr size_t kWorkspaceBytes = kCounterBytes + sizeof(PartialTile) * kMaxTeams * 2;
 
 struct DecodeParams {
   HeadRows q;
@@ -45,374 +52,515 @@ struct DecodeParams {
   const int* page_table;
   const int* seq_lens;
   char* out;
-  int* counters;               // one per block: arrivals at the sequence that the block ends within
+  int* counters;               // one per team: arrivals at the item that the team ends within
   PartialTile* partials;
   int* index_word;
   int batch, q_heads, kv_heads, dim;
-  int group, row_tiles;        // query heads per head of keys, tiles of rows they take
+  int group, row_tiles, items;         // query heads per head of keys, tiles of rows they take, items of a sequence
+  int solo_tiles;                      // tiles up to which a warp takes an item of a sequence alone
   int table_pages, pages;
-  long long capacity;          // tokens that a row of the table has room for
+  int capacity;                        // tokens that a row of the table has room for
   float scale_log2;
   FastDiv by_page;
 };
 
-// DP: head size rounded up.  HALF: at most eight rows are in use.
-template <typename T, int DP, bool HALF>
+// DP: head size rounded up.  HALF: at most eight rows are in use.  EIGHTS: pages of a multiple of eight tokens.
+template <typename T, int DP, bool HALF, bool EIGHTS>
 struct Decode {
-  static constexpr int kKeys = DP <= 64 ? 32 : 16;            // keys per warp and tile: 8 KB of keys and values
-  static constexpr int kStepKeys = kKeys * kWarps;
-  static constexpr int kPieces = DP / 8;                      // of 16 bytes per row
-  static constexpr int kSideBytes = kKeys * DP * 2;
+  static constexpr int kBoxes = DP / 64;                      // of 64 columns, rows of 128 bytes
+  static constexpr int kKeys = DP == 64 ? 32 : 16;            // keys per tile: 8 KB of keys and values
+  static constexpr int kSideBytes = kKeys * 128 * kBoxes;
   static constexpr int kTileBytes = 2 * kSideBytes;
-  static constexpr int kRingBytes = kWarps * kStages * kTileBytes;
-  static constexpr int kJoinBytes = kWarps * 8 * DP * 4;      // eight rows of every warp's output
-  static constexpr int kSmem = kRingBytes + kJoinBytes;
+  static constexpr int kRingBytes = kTeamWarps * kTeams * kStages * kTileBytes;
+  // eight rows of every warp's output, maximum and sum; rows eight banks apart, so that a warp's stores meet no conflict
+  static constexpr int kJoinRow = DP + 8;
+  static constexpr int kJoinBytes = kTeamWarps * 8 * kJoinRow * 4;
+  static constexpr int kSmem = kRingBytes + kTeams * kJoinBytes;
 };
 
-struct Item {          // a sequence, a head of keys and a tile of its query heads
-  int seq, head, row_tile, len;
+// An item, or four whose warps take one each, and the steps of it that are in turn.
+struct Cursor {
+  int seq, unit, len, step, stop;      // stop < 0: the run is over
+  bool solo;
+};
+// Runs of a list of n units over `count` takers: the first n % count have one more.
+struct Cut {
+  unsigned each, more;
+  __device__ __forceinline__ Cut(unsigned n, unsigned count) : each(n / count), more(n - n / count * count) {}
+  __device__ __forceinline__ unsigned begin(unsigned i) const { return i * each + min(i, more); }
+  __device__ __forceinline__ unsigned taker(unsigned at) const {
+    const unsigned low = more * (each + 1);
+    return at < low ? at / (each + 1) : more + (at - low) / each;
+  }
 };
 
-template <typename T, int DP, bool HALF>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(const DecodeParams p) {
-  using C = Decode<T, DP, HALF>;
+template <typename T, int DP, bool HALF, bool EIGHTS>
+__global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeParams p) {
+  using C = Decode<T, DP, HALF, EIGHTS>;
   extern __shared__ __align__(128) char smem[];
-  __shared__ float s_m[kWarps][kRows], s_sum[kWarps][kRows];
-  __shared__ int s_last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ unsigned s_warp[kThreads / 32];
+  __shared__ int s_place[kTeams][2][3];        // of a team: where its run begins and ends -- sequence, item, step
+  __shared__ int s_last[kTeams];
+  unsigned* s_scan = reinterpret_cast<unsigned*>(smem + C::kRingBytes);       // (where joins are, later)
+  const int warp = tc::uniform_warp(), lane = threadIdx.x & 31, team = warp / kTeamWarps, member = warp % kTeamWarps;
+  // the runs of the list go to the blocks' first teams, then to their second ones
+  const int runs = gridDim.x * kTeams, run = blockIdx.x + team * gridDim.x;
   chain_wait();
   chain_release();
 
-  // ---- this block's run of steps.  Every warp adds up the lengths, 1/32 of them to a lane.
+  // ---- the list's length and where runs begin.  A thread has 1/256 of the batch.
   auto length_of = [&](int seq) {
     int n = __ldg(p.seq_lens + seq);
-    if (n < 0 || n > p.capacity) {
+    if (static_cast<unsigned>(n) > static_cast<unsigned>(p.capacity)) {
       if (p.index_word) *p.index_word = kBadIndex;
-      n = n < 0 ? 0 : static_cast<int>(p.capacity);
+      n = n < 0 ? 0 : p.capacity;
     }
     return n;
   };
-  auto steps_of = [&](int len) { return max(1, (len + C::kStepKeys - 1) / C::kStepKeys); };
-  const int heads = p.kv_heads * p.row_tiles;                 // items of a sequence
-  const int slice = (p.batch + 31) / 32, lo = min(lane * slice, p.batch), hi = min(lo + slice, p.batch);
-  long long mine = 0;
-  for (int s = lo; s < hi; ++s) mine += steps_of(length_of(s));
-  long long before = mine;                                    // of this lane's slice and those in front of it
+  auto tiles_of = [&](int len) { return max(1, (len + C::kKeys - 1) / C::kKeys); };
+  auto is_solo = [&](int tiles) { return tiles <= p.solo_tiles; };
+  auto steps_of = [&](int tiles) { return is_solo(tiles) ? tiles : (tiles + kTeamWarps - 1) / kTeamWarps; };
+  auto units_of = [&](int tiles) { return is_solo(tiles) ? (p.items + kTeamWarps - 1) / kTeamWarps : p.items; };
+  const int slice = (p.batch + kThreads - 1) / kThreads;
+  unsigned sum_cost = 0;
+  float about = 0.0f;
+#pragma unroll 1
+  for (int s = threadIdx.x * slice, n = 0; n < slice && s < p.batch; ++s, ++n) {
+    const int tiles = tiles_of(length_of(s));
+    const unsigned cost = static_cast<unsigned>(steps_of(tiles) + kItemCost) * units_of(tiles);
+    sum_cost += cost;
+    about += static_cast<float>(cost);
+  }
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long other = __shfl_up_sync(0xffffffffu, before, d);
-    if (lane >= d) before += other;
+    const unsigned other = __shfl_up_sync(0xffffffffu, sum_cost, d);
+    if (lane >= d) sum_cost += other;
   }
-  const long long total = __shfl_sync(0xffffffffu, before, 31) * heads;
-  const long long wanted = (total + kMinSteps - 1) / kMinSteps;
-  const long long grid = wanted < gridDim.x ? wanted : gridDim.x;
-  if (blockIdx.x >= grid) return;
-  long long at = total * blockIdx.x / grid;
-  const long long end = total * (blockIdx.x + 1) / grid;
-
-  // the item that step `at` is in, and its first step
-  Item item;
-  long long item_begin;
-  {
-    const bool here = before * heads > at;
-    const int who = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-    long long base = before - mine;
-    int s = lo;
-    if (lane == who) {
-      while ((base + steps_of(length_of(s))) * heads <= at) base += steps_of(length_of(s++));
+  s_scan[threadIdx.x] = sum_cost;
+  if (lane == 31) s_warp[warp] = sum_cost;
+  // sums have 31 bits: a slice of 2^23 steps, 272 GB of keys and values, is refused
+  if (__syncthreads_or(about > 8388607.0f)) {
+    if (p.index_word) *p.index_word = kBadIndex;
+    return;
+  }
+  unsigned total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) total += s_warp[w];
+  const Cut cut(total, runs);
+  if (member == 0 && lane < 2) {
+    unsigned rest = cut.begin(run + lane);
+    const bool behind = rest >= total;                         // behind the last item
+    if (behind) rest = total - 1;
+    int w = 0;
+    while (rest >= s_warp[w]) rest -= s_warp[w++];
+    int t = 0;                                                 // the first thread of the warp whose sum is above `rest`
+#pragma unroll
+    for (int d = 16; d; d >>= 1)
+      if (s_scan[w * 32 + t + d - 1] <= rest) t += d;
+    if (t) rest -= s_scan[w * 32 + t - 1];
+    int seq = (w * 32 + t) * slice;
+    unsigned cost;
+    int tiles;
+    for (;; ++seq) {
+      tiles = tiles_of(length_of(seq));
+      cost = steps_of(tiles) + kItemCost;
+      if (rest < cost * units_of(tiles)) break;
+      rest -= cost * units_of(tiles);
     }
-    base = __shfl_sync(0xffffffffu, base, who);
-    s = __shfl_sync(0xffffffffu, s, who);
-    item.seq = s;
-    item.len = length_of(s);
-    const int h = static_cast<int>((at - base * heads) / steps_of(item.len));
-    item.head = h / p.row_tiles;
-    item.row_tile = h - item.head * p.row_tiles;
-    item_begin = base * heads + static_cast<long long>(h) * steps_of(item.len);
+    int unit = static_cast<int>(rest / cost), step = 0;
+    rest -= unit * cost;
+    if (behind) ++unit;
+    else if (!is_solo(tiles) && cost > kWholeSteps + kItemCost) step = max(0, static_cast<int>(rest) - kItemCost);
+    else if (2 * rest >= cost) ++unit;                         // the place moves to where an item begins
+    s_place[team][lane][0] = seq;
+    s_place[team][lane][1] = unit;
+    s_place[team][lane][2] = step;
   }
-  auto next_item = [&](Item& it) {
-    if (++it.row_tile < p.row_tiles) return;
-    it.row_tile = 0;
-    if (++it.head < p.kv_heads) return;
-    it.head = 0;
-    if (++it.seq < p.batch) it.len = length_of(it.seq);
-  };
+  __syncthreads();
+  const int end_seq = s_place[team][1][0], end_unit = s_place[team][1][1], end_step = s_place[team][1][2];
 
-  // ---- copies: this warp's tile of a step, lanes 0-15 know the keys' rows and lanes 16-31 the values' (two each at D <= 64)
-  const uint32_t ring = tc::smem_u32(smem) + warp * (kStages * C::kTileBytes);
-  Item load_item = item;
-  long long load_at = at, load_begin = item_begin;
-  int load_stage = 0;
-  auto issue = [&]() {
-    if (load_at < end) {
-      const int key0 = (static_cast<int>(load_at - load_begin) * kWarps + warp) * C::kKeys;
-      constexpr int kPer = C::kKeys / 16;
-      const CacheSide& side = lane < 16 ? p.kc : p.vc;
-      const char* base[kPer];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int key = key0 + i * 16 + (lane & 15);
-        base[i] = nullptr;
-        if (key < load_item.len) {
-          const int slot = fast_div(key, p.by_page), offset = key - slot * static_cast<int>(p.by_page.d);
-          const int page = __ldg(p.page_table + static_cast<long long>(load_item.seq) * p.table_pages + slot);
-          if (page < 0 || page >= p.pages) {
-            if (p.index_word) *p.index_word = kBadIndex;
-          } else {
-            base[i] = side.data + page * side.page_stride + load_item.head * side.head_stride + offset * side.token_stride;
-          }
-        }
+  // from the place the cursor is at to what is there, or next
+  auto settle = [&](Cursor& c) {
+    c.stop = -1;
+#pragma unroll 1
+    while (c.seq <= end_seq && c.seq < p.batch) {
+      c.len = length_of(c.seq);
+      const int tiles = tiles_of(c.len);
+      if (c.unit < units_of(tiles)) {
+        if (c.seq == end_seq && c.unit > end_unit) return;
+        const int stop = c.seq == end_seq && c.unit == end_unit ? end_step : steps_of(tiles);
+        if (c.step < stop) c.stop = stop;
+        c.solo = is_solo(tiles);
+        return;
       }
-      const uint32_t dst = ring + load_stage * C::kTileBytes;
-      // 32 pieces per instruction: rows of 16, 12 or 8 pieces
-      constexpr int kCopies = C::kKeys * C::kPieces / 32;
+      c.unit = 0;
+      ++c.seq;
+    }
+  };
+  auto advance = [&](Cursor& c) {
+    ++c.unit;
+    c.step = 0;
+    settle(c);
+  };
+  auto item_of = [&](const Cursor& c) { return c.solo ? c.unit * kTeamWarps + member : c.unit; };       // p.items or more: none
+  auto tile_of = [&](const Cursor& c) { return c.solo ? c.step : c.step * kTeamWarps + member; };
+  auto keys_of = [&](const Cursor& c) { return item_of(c) < p.items ? min(C::kKeys, c.len - tile_of(c) * C::kKeys) : 0; };
+  auto head_of = [&](int item) { return p.row_tiles == 1 ? item : item / p.row_tiles; };
+  Cursor next{s_place[team][0][0], s_place[team][0][1], 0, s_place[team][0][2], -1, false};
+  settle(next);
+
+  // ---- copies of this warp's next tile
+  const uint32_t ring = tc::smem_u32(smem) + warp * (kStages * C::kTileBytes);
+  Cursor load = next;
+  int load_stage = 0, page = -1, offset = 0;
+  // EIGHTS: the page of this lane's eight rows of the tile that is copied next, looked up a turn ahead
+  auto look_up = [&]() {
+    if (!EIGHTS || load.stop < 0 || lane * 8 >= keys_of(load)) return;
+    const int key = tile_of(load) * C::kKeys + lane * 8, slot = fast_div(key, p.by_page);
+    offset = key - slot * static_cast<int>(p.by_page.d);
+    page = __ldg(p.page_table + static_cast<long long>(load.seq) * p.table_pages + slot);
+  };
+  look_up();
+  constexpr int kPieces = C::kBoxes * 8, kRowsPerCopy = 32 / kPieces;        // of 16 bytes to a row; rows that a warp copies at a time
+  const int lane_row = lane / kPieces, lane_piece = lane % kPieces;
+  const long long k_lane = lane_row * p.kc.token_stride + lane_piece * 16, v_lane = lane_row * p.vc.token_stride + lane_piece * 16;
+  const bool in_head = lane_piece * 8 < p.dim;
+  auto issue = [&]() {
+    if (load.stop >= 0) {
+      const int key0 = tile_of(load) * C::kKeys, keys = keys_of(load), head = head_of(item_of(load));
+      // rows behind the sequence's end are not read and become zero: their weights are, and 0 x NaN would be NaN
+      const uint32_t dst = ring + load_stage * C::kTileBytes + (lane_piece >> 3) * C::kKeys * 128 + lane_row * 128;
+      const char* k_head = p.kc.data + head * p.kc.head_stride;
+      const char* v_head = p.vc.data + head * p.vc.head_stride;
+      auto copy = [&](int row0, const char* k_src, const char* v_src, bool there) {
+        const bool valid = there && row0 + lane_row < keys && in_head;
+        const uint32_t at = dst + row0 * 128 + ((((lane_piece & 7) ^ ((row0 + lane_row) & 7))) << 4);
+        copy16_async(at, valid ? k_src : p.kc.data, valid);
+        copy16_async(at + C::kSideBytes, valid ? v_src : p.vc.data, valid);
+      };
+      if (EIGHTS) {
+        const bool bad = lane * 8 < keys && static_cast<unsigned>(page) >= static_cast<unsigned>(p.pages);
+        if (bad && p.index_word) *p.index_word = kBadIndex;
+        const int good_page = bad ? -1 : page;
 #pragma unroll
-      for (int sidx = 0; sidx < 2; ++sidx) {
+        for (int e = 0; e < C::kKeys / 8; ++e) {
+          const int at_page = __shfl_sync(0xffffffffu, good_page, e), at_row = __shfl_sync(0xffffffffu, offset, e);
+          const char* k_src = k_head + at_page * p.kc.page_stride + at_row * p.kc.token_stride + k_lane;
+          const char* v_src = v_head + at_page * p.vc.page_stride + at_row * p.vc.token_stride + v_lane;
 #pragma unroll
-        for (int c = 0; c < kCopies; ++c) {
-          const int i = c * 32 + lane, row = i / C::kPieces, piece = i - row * C::kPieces;
-          const int from = sidx * 16 + (row & 15);
-          unsigned long long src = 0;
+          for (int r = 0; r < 8; r += kRowsPerCopy)
+            copy(e * 8 + r, k_src + r * p.kc.token_stride, v_src + r * p.vc.token_stride, at_page >= 0);
+        }
+      } else {
+        const int* table = p.page_table + static_cast<long long>(load.seq) * p.table_pages;
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            const unsigned long long v = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(base[j]), from);
-            if (j == row / 16) src = v;
+        for (int r = 0; r < C::kKeys; r += kRowsPerCopy) {
+          int at_page = -1, at_row = 0;
+          if (r + lane_row < keys) {
+            const int key = key0 + r + lane_row, slot = fast_div(key, p.by_page);
+            at_row = key - slot * static_cast<int>(p.by_page.d);
+            at_page = __ldg(table + slot);
+            if (static_cast<unsigned>(at_page) >= static_cast<unsigned>(p.pages)) {
+              if (p.index_word) *p.index_word = kBadIndex;
+              at_page = -1;
+            }
           }
-          const bool valid = src != 0 && piece * 8 < p.dim;
-          copy16_async(dst + sidx * C::kSideBytes + piece_at<DP>(row, piece),
-                       valid ? reinterpret_cast<const char*>(src) + piece * 16 : p.kc.data, valid);
+          copy(r, k_head + at_page * p.kc.page_stride + at_row * p.kc.token_stride + lane_piece * 16,
+               v_head + at_page * p.vc.page_stride + at_row * p.vc.token_stride + lane_piece * 16, at_page >= 0);
         }
       }
       if (++load_stage == kStages) load_stage = 0;
-      ++load_at;
-      if (load_at - load_begin == steps_of(load_item.len)) {
-        load_begin = load_at;
-        next_item(load_item);
-      }
+      if (++load.step >= load.stop) advance(load);
+      look_up();
     }
     copies_commit();
   };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue();
 
   constexpr int kNT = DP / 8;                                  // 8-column tiles of the output
   constexpr int kHalves = HALF ? 1 : 2;                        // rows lane / 4 and lane / 4 + 8
-  int stage = 0;
   const int row0 = lane >> 2, col0 = (lane & 3) * 2;
-  while (at < end) {
-    // ---- one item, or this block's part of it
-    const long long item_end = item_begin + steps_of(item.len);
-    const int steps = static_cast<int>((item_end < end ? item_end : end) - at);
-    const int row_base = item.head * p.group + item.row_tile * kRows;       // query head of row 0
-    const int rows = min(kRows, p.group - item.row_tile * kRows);
-    uint32_t qf[DP / 16][4];
-    {
-      const char* q = p.q.data + item.seq * p.q.token_stride + row_base * p.q.head_stride;
+  int stage = 0;
+  uint32_t qf[DP / 16][4], q_next[DP / 16][2 * kHalves];
+  float o[kNT][4], m[2], sum[2];
+  auto row_tile = [&](int item) { return item - head_of(item) * p.row_tiles; };
+  auto rows_of = [&](int item) { return item < p.items ? min(kRows, p.group - row_tile(item) * kRows) : 0; };
+  auto first_row = [&](int item) { return head_of(item) * p.group + row_tile(item) * kRows; };
+  // Queries as the products' left operand: registers [k][0] and [2] are row lane / 4, [1] and [3] row lane / 4 + 8.  The next
+  // item's are fetched while one is run.
+  auto fetch_q = [&](const Cursor& c) {
+    if (c.stop < 0) return;
+    const int item = item_of(c), rows = rows_of(item);
+    const char* q = p.q.data + c.seq * p.q.token_stride + first_row(item) * p.q.head_stride;
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k)
+    for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = row0 + (j & 1) * 8, c = k * 16 + col0 + (j >> 1) * 8;
-          qf[k][j] = (HALF && (j & 1)) || r >= rows || c >= p.dim
-                         ? 0u : __ldg(reinterpret_cast<const unsigned int*>(q + r * p.q.head_stride + c * 2));
-        }
-    }
-    float o[kNT][4];
-#pragma unroll
-    for (int n = 0; n < kNT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-    float m[2] = {kNegInf, kNegInf}, sum[2] = {0.0f, 0.0f};
+      for (int j = 0; j < 2 * kHalves; ++j) {
+        const int r = row0 + (HALF ? 0 : (j & 1) * 8), col = k * 16 + col0 + (HALF ? j : j >> 1) * 8;
+        q_next[k][j] = r >= rows || col >= p.dim ? 0u : __ldg(reinterpret_cast<const unsigned int*>(q + r * p.q.head_stride + col * 2));
+      }
+  };
+  auto row_of = [&](const Cursor& c, int item, int row) {
+    return p.out + (static_cast<long long>(c.seq) * p.q_heads + first_row(item) + row) * p.dim * 2;
+  };
+  auto store = [&](const Cursor& c, int row, int col, float4 v, float sum) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<uint2*>(row_of(c, c.unit, row) + col * 2) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+  };
+  auto team_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kTeam) : "memory"); };
 
-    int key0 = (static_cast<int>(at - item_begin) * kWarps + warp) * C::kKeys;
-    for (int step = 0; step < steps; ++step, key0 += C::kStepKeys) {
-      issue();
-      copies_wait<kStages - 1>();
-      __syncwarp();
-      const uint32_t tile_k = ring + stage * C::kTileBytes, tile_v = tile_k + C::kSideBytes;
-      if (++stage == kStages) stage = 0;
-      if (key0 < item.len) {
-        constexpr int kST = C::kKeys / 8;
-        float s[kST][4];
-#pragma unroll
-        for (int n = 0; n < kST; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-          for (int n = 0; n < kST / 2; ++n) {
-            uint32_t b[4];
-            ldmatrix_x4(b, tile_k + piece_at<DP>(n * 16 + (lane & 7) + (lane >> 4) * 8, k * 2 + ((lane >> 3) & 1)));
-            mma_16816<T>(s[2 * n], qf[k], b[0], b[1]);
-            mma_16816<T>(s[2 * n + 1], qf[k], b[2], b[3]);
-          }
-        const int left = item.len - key0;
-        float keep[2] = {1.0f, 1.0f}, base[2];
+  // ---- The turns of the loop: the first ones only copy; at an item's end it is joined and the next one begun; else a tile.
+  float* join = reinterpret_cast<float*>(smem + C::kRingBytes + team * C::kJoinBytes);
+  const int thread = threadIdx.x % kTeam;
+  fetch_q(next);
+  Cursor now{0, 0, 0, 0, 0, false};
+  int first_step = 0, ahead = kStages - 1;
+  bool running = false;
+#pragma unroll 1
+  for (;;) {
+    if (ahead == 0 && now.step >= now.stop) {
+      if (running) {
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-          float top = kNegInf;
-#pragma unroll
-          for (int n = 0; n < kST; ++n)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float& v = s[n][2 * h + j];
-              v = n * 8 + col0 + j < left ? v * p.scale_log2 : kNegInf;
-              top = fmaxf(top, v);
-            }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float now = fmaxf(m[h], top);
-          base[h] = now == kNegInf ? 0.0f : now;         // nothing but minus infinity yet: no difference of infinities
-          keep[h] = exp2_fast(m[h] - base[h]);
-          m[h] = now;
-          sum[h] *= keep[h];
+          sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+          sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
         }
-        uint32_t pf[kST / 2][4];
+      }
+      if (running && now.solo) {
+        const int item = item_of(now);
 #pragma unroll
-        for (int n = 0; n < kST; ++n)
+        for (int h = 0; h < kHalves; ++h) {
+          const int row = row0 + 8 * h;
+          if (row >= rows_of(item)) continue;
+          const float inv = sum[h] == 0.0f ? 0.0f : 1.0f / sum[h];
+          char* dst = row_of(now, item, row);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h < kHalves) {
-              const float e0 = exp2_fast(s[n][2 * h] - base[h]), e1 = exp2_fast(s[n][2 * h + 1] - base[h]);
-              sum[h] += e0 + e1;
-              pf[n >> 1][(n & 1) * 2 + h] = pack2<T>(e0, e1);
+          for (int n = 0; n < kNT; ++n)
+            if (n * 8 + col0 < p.dim)
+              *reinterpret_cast<uint32_t*>(dst + (n * 8 + col0) * 2) = pack2<T>(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
+        }
+      } else if (running) {
+        const int rows = rows_of(now.unit), all = steps_of(tiles_of(now.len));
+        const bool enters = first_step > 0, leaves = now.stop < all;
+        PartialTile* part = p.partials + (run * 2 + (enters ? 0 : 1));
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          team_sync();                         // what was there has been read
+          float* own = join + (member * 8 + row0) * C::kJoinRow;
+#pragma unroll
+          for (int n = 0; n < kNT; ++n) *reinterpret_cast<float2*>(own + n * 8 + col0) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+          if ((lane & 3) == 0) *reinterpret_cast<float2*>(own + DP) = make_float2(m[h], sum[h]);
+          team_sync();
+#pragma unroll 1
+          for (int i = thread; i < 8 * DP / 4; i += kTeam) {
+            const int r = i / (DP / 4), col = (i - r * (DP / 4)) * 4, row = r + 8 * h;
+            if (row >= rows) break;
+            float2 of[kTeamWarps];             // maximum and sum
+            float top = kNegInf, row_sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kTeamWarps; ++w) {
+              of[w] = *reinterpret_cast<const float2*>(join + (w * 8 + r) * C::kJoinRow + DP);
+              top = fmaxf(top, of[w].x);
+            }
+            const float base = top == kNegInf ? 0.0f : top;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kTeamWarps; ++w) {
+              const float f = exp2_fast(of[w].x - base);
+              const float4 x = *reinterpret_cast<const float4*>(join + (w * 8 + r) * C::kJoinRow + col);
+              acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+              row_sum += of[w].y * f;
+            }
+            if (!enters && !leaves) {
+              if (col < p.dim) store(now, row, col, acc, row_sum);
             } else {
-              pf[n >> 1][(n & 1) * 2 + h] = 0u;
+              __stcg(reinterpret_cast<float4*>(&part->o[row][col]), acc);
+              if (col == 0) {
+                __stcg(&part->m[row], top);
+                __stcg(&part->sum[row], row_sum);
+              }
             }
           }
-#pragma unroll
-        for (int n = 0; n < kNT; ++n)
-#pragma unroll
-          for (int h = 0; h < kHalves; ++h) {
-            o[n][2 * h] *= keep[h];
-            o[n][2 * h + 1] *= keep[h];
+        }
+        if (enters || leaves) {
+          // ---- an item that spans teams: whoever arrives last joins the parts
+          const unsigned first_unit = enters ? cut.begin(run) - first_step : cut.begin(run + 1) - now.stop;
+          const int first = static_cast<int>(cut.taker(first_unit)), last = static_cast<int>(cut.taker(first_unit + all - 1));
+          team_sync();
+          if (thread == 0) {
+            __threadfence();
+            s_last[team] = atomicAdd(p.counters + first, 1) == last - first;
+            if (s_last[team]) p.counters[first] = 0;
+            __threadfence();
           }
+          team_sync();
+          if (s_last[team]) {
+#pragma unroll 1
+            for (int i = thread; i < rows * (DP / 4); i += kTeam) {
+              const int row = i / (DP / 4), col = (i - row * (DP / 4)) * 4;
+              if (col >= p.dim) continue;
+              float top = kNegInf, row_sum = 0.0f;
+              float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              constexpr int kBatch = 8;        // parts that are fetched at a time
+#pragma unroll 1
+              for (int t0 = first; t0 <= last; t0 += kBatch) {
+                float pm[kBatch], ps[kBatch];
+                float4 po[kBatch];
 #pragma unroll
-        for (int k = 0; k < kST / 2; ++k)
+                for (int e = 0; e < kBatch; ++e) {
+                  const int t = min(t0 + e, last);
+                  const PartialTile& x = p.partials[t * 2 + (t == first)];
+                  pm[e] = t0 + e <= last ? __ldcg(&x.m[row]) : kNegInf;
+                  ps[e] = __ldcg(&x.sum[row]);
+                  po[e] = __ldcg(reinterpret_cast<const float4*>(&x.o[row][col]));
+                }
+                float higher = top;
 #pragma unroll
-          for (int n = 0; n < kNT / 2; ++n) {
-            uint32_t b[4];
-            ldmatrix_x4_trans(b, tile_v + piece_at<DP>(k * 16 + (lane & 15), n * 2 + (lane >> 4)));
-            mma_16816<T>(o[2 * n], pf[k], b[0], b[1]);
-            mma_16816<T>(o[2 * n + 1], pf[k], b[2], b[3]);
+                for (int e = 0; e < kBatch; ++e) higher = fmaxf(higher, pm[e]);
+                const float base = higher == kNegInf ? 0.0f : higher, keep = exp2_fast(top - base);
+                top = higher;
+                row_sum *= keep;
+                acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e) {
+                  if (t0 + e > last) break;
+                  const float f = exp2_fast(pm[e] - base);
+                  row_sum += ps[e] * f;
+                  acc.x += po[e].x * f; acc.y += po[e].y * f; acc.z += po[e].z * f; acc.w += po[e].w * f;
+                }
+              }
+              store(now, row, col, acc, row_sum);
+            }
           }
+        }
       }
-      __syncwarp();            // the next copies overwrite this tile
-    }
-
-    // ---- the block's four warps
+      if (next.stop < 0) break;
+      now = next;
+      first_step = now.step;
+      running = true;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-      if ((lane & 3) == 0) {
-        s_m[warp][row0 + 8 * h] = m[h];
-        s_sum[warp][row0 + 8 * h] = sum[h];
+      for (int k = 0; k < DP / 16; ++k) {
+        qf[k][0] = q_next[k][0];
+        qf[k][1] = HALF ? 0u : q_next[k][HALF ? 0 : 1];
+        qf[k][2] = q_next[k][HALF ? 1 : 2];
+        qf[k][3] = HALF ? 0u : q_next[k][HALF ? 0 : 3];
       }
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+      m[0] = m[1] = kNegInf;
+      sum[0] = sum[1] = 0.0f;
+      advance(next);
+      fetch_q(next);
     }
-    __syncthreads();
-    const bool whole = at == item_begin && item_end <= end;
-    PartialTile* part = p.partials + (blockIdx.x * 2 + (at == item_begin ? 1 : 0));
-    float* join = reinterpret_cast<float*>(smem + C::kRingBytes);
+    issue();
+    if (ahead) {
+      --ahead;
+      continue;
+    }
+    const int keys = keys_of(now);
+    const uint32_t tile_k = ring + stage * C::kTileBytes, tile_v = tile_k + C::kSideBytes;
+    copies_wait<kStages - 1>();
+    __syncwarp();
+    if (++stage == kStages) stage = 0;
+    ++now.step;
+    if (keys <= 0) continue;
+    constexpr int kST = C::kKeys / 8;
+    float s[kST][4], odd[kST][4];              // products of even and odd sixteens of the head: two shorter chains
+#pragma unroll
+    for (int n = 0; n < kST; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = odd[n][e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+      for (int n = 0; n < kST / 2; ++n) {
+        uint32_t b[4];
+        const int row = n * 16 + (lane & 7) + (lane >> 4) * 8;
+        ldmatrix_x4(b, tile_k + (k >> 2) * C::kKeys * 128 + row * 128 + ((((k & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+        mma_16816<T>(k & 1 ? odd[2 * n] : s[2 * n], qf[k], b[0], b[1]);
+        mma_16816<T>(k & 1 ? odd[2 * n + 1] : s[2 * n + 1], qf[k], b[2], b[3]);
+      }
+    float base[2], top[2];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
-      float top = kNegInf;
+      top[h] = m[h];
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][row0 + 8 * h]);
-      const float scale = exp2_fast(m[h] - (top == kNegInf ? 0.0f : top));
+      for (int n = 0; n < kST; ++n)
 #pragma unroll
-      for (int n = 0; n < kNT; ++n)
-        *reinterpret_cast<float2*>(join + (warp * 8 + row0) * DP + n * 8 + col0) = make_float2(o[n][2 * h] * scale, o[n][2 * h + 1] * scale);
-      __syncthreads();
-      for (int i = threadIdx.x; i < 8 * DP / 4; i += kThreads) {
-        const int r = i / (DP / 4), c = (i - r * (DP / 4)) * 4, row = r + 8 * h;
-        if (row >= rows) break;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float row_top = kNegInf, row_sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) row_top = fmaxf(row_top, s_m[w][row]);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(join + (w * 8 + r) * DP + c);
-          acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
-          row_sum += s_sum[w][row] * exp2_fast(s_m[w][row] - (row_top == kNegInf ? 0.0f : row_top));
+        for (int j = 0; j < 2; ++j) {
+          float& v = s[n][2 * h + j];
+          v = n * 8 + col0 + j < keys ? (v + odd[n][2 * h + j]) * p.scale_log2 : kNegInf;
+          top[h] = fmaxf(top[h], v);
         }
-        if (whole) {
-          if (c < p.dim) {
-            const float inv = row_sum == 0.0f ? 0.0f : 1.0f / row_sum;
-            char* dst = p.out + ((static_cast<long long>(item.seq) * p.q_heads + row_base + row) * p.dim + c) * 2;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-          }
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+    }
+    if (__any_sync(0xffffffffu, top[0] > m[0] || (!HALF && top[kHalves - 1] > m[kHalves - 1]))) {
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const float keep = top[h] == kNegInf ? 1.0f : exp2_fast(m[h] - top[h]);
+        m[h] = top[h];
+        sum[h] *= keep;
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          o[n][2 * h] *= keep;
+          o[n][2 * h + 1] *= keep;
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) base[h] = m[h] == kNegInf ? 0.0f : m[h];   // nothing but minus infinity yet: no difference
+    uint32_t pf[kST / 2][4];                                                     // of infinities
+#pragma unroll
+    for (int n = 0; n < kST; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h < kHalves) {
+          const float e0 = exp2_fast(s[n][2 * h] - base[h]), e1 = exp2_fast(s[n][2 * h + 1] - base[h]);
+          sum[h] += e0 + e1;
+          pf[n >> 1][(n & 1) * 2 + h] = pack2<T>(e0, e1);
         } else {
-          __stcg(reinterpret_cast<float4*>(&part->o[row][c]), acc);
-          if (c == 0) {
-            __stcg(&part->m[row], row_top);
-            __stcg(&part->sum[row], row_sum);
-          }
+          pf[n >> 1][(n & 1) * 2 + h] = 0u;
         }
       }
-      __syncthreads();
-    }
-
-    // ---- a sequence that spans blocks: whoever arrives last joins the parts
-    if (!whole) {
-      const long long last_step = item_end - 1;
-      const int first = static_cast<int>(((item_begin + 1) * grid - 1) / total);
-      const int last = static_cast<int>(((last_step + 1) * grid - 1) / total);
-      if (threadIdx.x == 0) {
-        __threadfence();
-        const int n = atomicAdd(p.counters + first, 1);
-        s_last = n == last - first;
-        if (s_last) p.counters[first] = 0;
-        __threadfence();
+#pragma unroll
+    for (int k = 0; k < kST / 2; ++k)
+#pragma unroll
+      for (int n = 0; n < kNT / 2; ++n) {
+        uint32_t b[4];
+        const int row = k * 16 + (lane & 15), piece = n * 2 + (lane >> 4);
+        ldmatrix_x4_trans(b, tile_v + (n >> 2) * C::kKeys * 128 + row * 128 + (((piece & 7) ^ (lane & 7)) << 4));
+        mma_16816<T>(o[2 * n], pf[k], b[0], b[1]);
+        mma_16816<T>(o[2 * n + 1], pf[k], b[2], b[3]);
       }
-      __syncthreads();
-      if (s_last) {
-        for (int i = threadIdx.x; i < rows * (DP / 4); i += kThreads) {
-          const int row = i / (DP / 4), c = (i - row * (DP / 4)) * 4;
-          if (c >= p.dim) continue;
-          float top = kNegInf;
-          for (int b = first; b <= last; ++b) top = fmaxf(top, __ldcg(&p.partials[b * 2 + (b == first)].m[row]));
-          const float ref = top == kNegInf ? 0.0f : top;
-          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          float row_sum = 0.0f;
-          for (int b = first; b <= last; ++b) {
-            const PartialTile& t = p.partials[b * 2 + (b == first)];
-            const float f = exp2_fast(__ldcg(&t.m[row]) - ref);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(&t.o[row][c]));
-            row_sum += __ldcg(&t.sum[row]) * f;
-            acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
-          }
-          const float inv = row_sum == 0.0f ? 0.0f : 1.0f / row_sum;
-          char* dst = p.out + ((static_cast<long long>(item.seq) * p.q_heads + row_base + row) * p.dim + c) * 2;
-          *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-        }
-      }
-      __syncthreads();
-    }
-    at += steps;
-    item_begin = item_end;
-    next_item(item);
+    __syncwarp();              // the next copies overwrite this tile
   }
   copies_wait<0>();
 }
 
-template <typename T, int DP, bool HALF>
+template <typename T, int DP, bool HALF, bool EIGHTS>
 int launch_decode(const DecodeParams& p, int grid, cudaStream_t st) {
-  using C = Decode<T, DP, HALF>;
+  using C = Decode<T, DP, HALF, EIGHTS>;
   static thread_local int configured_device = -1;
   int device = 0;
   MP_CUDA_TRY(cudaGetDevice(&device));
   if (configured_device != device) {
-    MP_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<T, DP, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    MP_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<T, DP, HALF, EIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     configured_device = device;
   }
-  return launch_chained(paged_decode_kernel<T, DP, HALF>, dim3(grid), dim3(kThreads), C::kSmem, st, p);
+  return launch_chained(paged_decode_kernel<T, DP, HALF, EIGHTS>, dim3(grid), dim3(kThreads), C::kSmem, st, p);
 }
 
+template <typename T, int DP, bool EIGHTS>
+int dispatch_rows(const DecodeParams& p, int grid, cudaStream_t st) {
+  return p.group <= 8 ? launch_decode<T, DP, true, EIGHTS>(p, grid, st) : launch_decode<T, DP, false, EIGHTS>(p, grid, st);
+}
+template <typename T, int DP>
+int dispatch_pages(const DecodeParams& p, int grid, cudaStream_t st) {
+  return p.by_page.d % 8 == 0 ? dispatch_rows<T, DP, true>(p, grid, st) : dispatch_rows<T, DP, false>(p, grid, st);
+}
 template <typename T>
 int dispatch_decode(const DecodeParams& p, int grid, cudaStream_t st) {
-  const bool half = p.group <= 8;
-  if (p.dim <= 64) return half ? launch_decode<T, 64, true>(p, grid, st) : launch_decode<T, 64, false>(p, grid, st);
-  if (p.dim <= 96) return half ? launch_decode<T, 96, true>(p, grid, st) : launch_decode<T, 96, false>(p, grid, st);
-  return half ? launch_decode<T, 128, true>(p, grid, st) : launch_decode<T, 128, false>(p, grid, st);
+  return p.dim <= 64 ? dispatch_pages<T, 64>(p, grid, st) : dispatch_pages<T, 128>(p, grid, st);
 }
 
 }  // namespace
@@ -446,14 +594,18 @@ extern "C" int mp_paged_attention_decode(int dtype, const mp_head_rows* q, int B
   p.row_tiles = (p.group + kRows - 1) / kRows;
   p.table_pages = table_pages;
   p.pages = cache->pages;
+  p.items = p.kv_heads * p.row_tiles;
   const long long room = static_cast<long long>(table_pages) * cache->page_size;
-  p.capacity = room < 0x7fffff00LL ? room : 0x7fffff00LL;
+  p.capacity = static_cast<int>(room < 0x7fffff00LL ? room : 0x7fffff00LL);
   p.scale_log2 = scale * attn::kLog2e;
   p.by_page = make_fast_div(cache->page_size);
-  // no more blocks than there can be steps
-  const int step = D <= 64 ? Decode<__half, 64, true>::kStepKeys : Decode<__half, 128, true>::kStepKeys;
-  const long long steps = static_cast<long long>(B) * p.kv_heads * p.row_tiles * ((p.capacity + step - 1) / step);
-  const int grid = static_cast<int>(steps < kMaxGrid ? steps : kMaxGrid);
+  const int keys = D <= 64 ? Decode<__half, 64, true, true>::kKeys : Decode<__half, 128, true, true>::kKeys;
+  // with four items to a team and more, warps take those of short sequences alone
+  p.solo_tiles = static_cast<long long>(B) * p.items >= 4 * kMaxTeams ? kSoloTiles : 1;
+  // no more teams than there can be whole items and steps of what is cut
+  const long long steps = (p.capacity + keys * kTeamWarps - 1LL) / (keys * kTeamWarps);
+  const long long teams = static_cast<long long>(B) * p.items * (steps <= kWholeSteps ? 1 : steps);
+  const int grid = static_cast<int>(teams < kSmCount ? teams : kSmCount);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == 0 ? dispatch_decode<__half>(p, grid, st) : dispatch_decode<__nv_bfloat16>(p, grid, st);
 }
