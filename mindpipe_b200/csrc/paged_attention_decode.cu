@@ -3,9 +3,9 @@
 //   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   s_j = scale q . k_j,   m = max_j s_j
 //
 // with a running m, sum and o, in one pass over the cache: 2 len Hkv D 16-bit values per sequence, which HBM bounds.  The
-// query heads that share a head of keys are the rows of a 16-row matrix product, so keys and values are read once for all
-// of them (mma.sync: at HBM's rate an SM multiplies one 16 x 16 piece of the cache in about 10 clocks, far below what even
-// this path of the tensor cores takes; tcgen05's 128 rows would be 7/8 padding or more).
+// query heads that share a head of keys are the eight columns of the products S^T = K Q^T and O^T = V^T P^T, so keys and
+// values are read once for all of them (mma.sync: at HBM's rate an SM multiplies one 16 x 16 piece of the cache in about 10
+// clocks, far below what even this path of the tensor cores takes; tcgen05's 128 rows would be 7/8 padding or more).
 //
 // All lengths are known on the device only (a captured launch serves every later step), so the work is cut there: the list of
 // (sequence, head) items, each in steps of a few keys, is cut evenly over teams of four warps, two teams to an SM, so that
@@ -27,24 +27,24 @@ namespace {
 
 using namespace attn;
 
-constexpr int kTeamWarps = 4, kTeam = 32 * kTeamWarps, kTeams = 2;       // teams of a block
-constexpr int kThreads = kTeam * kTeams;
 constexpr int kStages = 3;
-constexpr int kMaxTeams = kSmCount * kTeams;
 constexpr int kRows = 16;                                     // query heads per tile
-constexpr int kMaxD = 128;
 constexpr int kItemCost = 2;           // what an item costs beside its steps, in steps
 constexpr int kWholeSteps = 4;         // steps up to which an item is not cut: a join of teams takes 2-3 us
 constexpr int kSoloTiles = 8;          // tiles of a sequence up to which a warp takes an item alone, if there are many items
 
 // A team's two parts of items that it shares: the one it begins within (0) and the one it ends within (1).
+template <int DP>
 struct PartialTile {
   float m[kRows], sum[kRows];
-  float o[kRows][kMaxD];
+  float o[kRows][DP];
 };
+template <int DP> constexpr int kWarpsOf = DP == 64 ? 16 : 8; // of a block, one block to an SM
+constexpr int kFour = 4;                                      // warps of a team where there are more items than blocks
 constexpr size_t kCounterBytes = 4096;
-static_assert(kMaxTeams * sizeof(int) <= kCounterBytes, "");
-constexpr size_t kWorkspaceBytes = kCounterBytes + sizeof(PartialTile) * kMaxTeams * 2;
+static_assert(kSmCount * kWarpsOf<64> / kFour * sizeof(int) <= kCounterBytes, "");
+template <int DP> constexpr size_t kPartialBytes = sizeof(PartialTile<DP>) * kSmCount * kWarpsOf<DP> / kFour * 2;
+constexpr size_t kWorkspaceBytes = kCounterBytes + (kPartialBytes<64> > kPartialBytes<128> ? kPartialBytes<64> : kPartialBytes<128>);
 
 struct DecodeParams {
   HeadRows q;
@@ -53,7 +53,7 @@ struct DecodeParams {
   const int* seq_lens;
   char* out;
   int* counters;               // one per team: arrivals at the item that the team ends within
-  PartialTile* partials;
+  void* partials;
   int* index_word;
   int batch, q_heads, kv_heads, dim;
   int group, row_tiles, items;         // query heads per head of keys, tiles of rows they take, items of a sequence
@@ -64,16 +64,19 @@ struct DecodeParams {
   FastDiv by_page;
 };
 
-// DP: head size rounded up.  HALF: at most eight rows are in use.  EIGHTS: pages of a multiple of eight tokens.
-template <typename T, int DP, bool HALF, bool EIGHTS>
+// DP: head size rounded up.  HALF: at most eight rows are in use.  EIGHTS: pages of a multiple of eight tokens.  WHOLE: the
+// block is one team.
+template <typename T, int DP, bool HALF, bool EIGHTS, bool WHOLE>
 struct Decode {
+  static constexpr int kTeamWarps = WHOLE ? kWarpsOf<DP> : kFour, kTeam = 32 * kTeamWarps;
+  static constexpr int kTeams = kWarpsOf<DP> / kTeamWarps, kThreads = kTeam * kTeams;
   static constexpr int kBoxes = DP / 64;                      // of 64 columns, rows of 128 bytes
-  static constexpr int kKeys = DP == 64 ? 32 : 16;            // keys per tile: 8 KB of keys and values
+  static constexpr int kKeys = 16;                            // per tile: 8 KB of keys and values, or 4
   static constexpr int kSideBytes = kKeys * 128 * kBoxes;
   static constexpr int kTileBytes = 2 * kSideBytes;
   static constexpr int kRingBytes = kTeamWarps * kTeams * kStages * kTileBytes;
-  // eight rows of every warp's output, maximum and sum; rows eight banks apart, so that a warp's stores meet no conflict
-  static constexpr int kJoinRow = DP + 8;
+  // eight rows of every warp's output, maximum and sum; rows four banks apart, so that a warp's stores meet no conflict
+  static constexpr int kJoinRow = DP + 4;
   static constexpr int kJoinBytes = kTeamWarps * 8 * kJoinRow * 4;
   static constexpr int kSmem = kRingBytes + kTeams * kJoinBytes;
 };
@@ -94,9 +97,19 @@ struct Cut {
   }
 };
 
-template <typename T, int DP, bool HALF, bool EIGHTS>
-__global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeParams p) {
-  using C = Decode<T, DP, HALF, EIGHTS>;
+// An 8 x 8 matrix of 16-bit values, two of a row to a lane, with rows and columns exchanged.
+__device__ __forceinline__ uint32_t transpose(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <typename T, int DP, bool HALF, bool EIGHTS, bool WHOLE>
+__global__ void __launch_bounds__(Decode<T, DP, HALF, EIGHTS, WHOLE>::kThreads, 1) paged_decode_kernel(const DecodeParams p) {
+  using C = Decode<T, DP, HALF, EIGHTS, WHOLE>;
+  constexpr int kTeams = C::kTeams, kThreads = C::kThreads, kTeamWarps = C::kTeamWarps, kTeam = C::kTeam;
+  using Partial = PartialTile<DP>;
+  Partial* const partials = static_cast<Partial*>(p.partials);
   extern __shared__ __align__(128) char smem[];
   __shared__ unsigned s_warp[kThreads / 32];
   __shared__ int s_place[kTeams][2][3];        // of a team: where its run begins and ends -- sequence, item, step
@@ -108,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
   chain_wait();
   chain_release();
 
-  // ---- the list's length and where runs begin.  A thread has 1/256 of the batch.
+  // ---- the list's length and where runs begin.  A thread has a slice of the batch.
   auto length_of = [&](int seq) {
     int n = __ldg(p.seq_lens + seq);
     if (static_cast<unsigned>(n) > static_cast<unsigned>(p.capacity)) {
@@ -212,26 +225,44 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
   // ---- copies of this warp's next tile
   const uint32_t ring = tc::smem_u32(smem) + warp * (kStages * C::kTileBytes);
   Cursor load = next;
-  int load_stage = 0, page = -1, offset = 0;
-  // EIGHTS: the page of this lane's eight rows of the tile that is copied next, looked up a turn ahead
-  auto look_up = [&]() {
-    if (!EIGHTS || load.stop < 0 || lane * 8 >= keys_of(load)) return;
-    const int key = tile_of(load) * C::kKeys + lane * 8, slot = fast_div(key, p.by_page);
-    offset = key - slot * static_cast<int>(p.by_page.d);
-    page = __ldg(p.page_table + static_cast<long long>(load.seq) * p.table_pages + slot);
+  int load_stage = 0;
+  // A tile that is to be copied: looks at the page table take as long as a copy, so they are made two turns ahead.
+  struct Ahead {
+    int seq, head, key0, keys;                 // keys < 0: there is none
+    int page, offset;                          // EIGHTS: of this lane's eight rows
   };
-  look_up();
+  auto look_up = [&]() {
+    Ahead t;
+    t.keys = -1;
+    if (load.stop < 0) return t;
+    t.seq = load.seq;
+    t.head = head_of(item_of(load));
+    t.key0 = tile_of(load) * C::kKeys;
+    t.keys = max(keys_of(load), 0);
+    t.page = t.offset = 0;
+    if (EIGHTS && lane * 8 < t.keys) {
+      const int key = t.key0 + lane * 8, slot = fast_div(key, p.by_page);
+      t.offset = key - slot * static_cast<int>(p.by_page.d);
+      t.page = __ldg(p.page_table + static_cast<long long>(t.seq) * p.table_pages + slot);
+    }
+    if (++load.step >= load.stop) advance(load);
+    return t;
+  };
+  Ahead first_up = look_up(), second_up = look_up();
   constexpr int kPieces = C::kBoxes * 8, kRowsPerCopy = 32 / kPieces;        // of 16 bytes to a row; rows that a warp copies at a time
   const int lane_row = lane / kPieces, lane_piece = lane % kPieces;
   const long long k_lane = lane_row * p.kc.token_stride + lane_piece * 16, v_lane = lane_row * p.vc.token_stride + lane_piece * 16;
   const bool in_head = lane_piece * 8 < p.dim;
   auto issue = [&]() {
-    if (load.stop >= 0) {
-      const int key0 = tile_of(load) * C::kKeys, keys = keys_of(load), head = head_of(item_of(load));
+    const Ahead t = first_up;
+    first_up = second_up;
+    second_up = look_up();
+    if (t.keys >= 0) {
+      const int keys = t.keys;
       // rows behind the sequence's end are not read and become zero: their weights are, and 0 x NaN would be NaN
       const uint32_t dst = ring + load_stage * C::kTileBytes + (lane_piece >> 3) * C::kKeys * 128 + lane_row * 128;
-      const char* k_head = p.kc.data + head * p.kc.head_stride;
-      const char* v_head = p.vc.data + head * p.vc.head_stride;
+      const char* k_head = p.kc.data + t.head * p.kc.head_stride;
+      const char* v_head = p.vc.data + t.head * p.vc.head_stride;
       auto copy = [&](int row0, const char* k_src, const char* v_src, bool there) {
         const bool valid = there && row0 + lane_row < keys && in_head;
         const uint32_t at = dst + row0 * 128 + ((((lane_piece & 7) ^ ((row0 + lane_row) & 7))) << 4);
@@ -239,12 +270,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
         copy16_async(at + C::kSideBytes, valid ? v_src : p.vc.data, valid);
       };
       if (EIGHTS) {
-        const bool bad = lane * 8 < keys && static_cast<unsigned>(page) >= static_cast<unsigned>(p.pages);
+        const bool bad = lane * 8 < keys && static_cast<unsigned>(t.page) >= static_cast<unsigned>(p.pages);
         if (bad && p.index_word) *p.index_word = kBadIndex;
-        const int good_page = bad ? -1 : page;
+        const int good_page = bad ? -1 : t.page;
 #pragma unroll
         for (int e = 0; e < C::kKeys / 8; ++e) {
-          const int at_page = __shfl_sync(0xffffffffu, good_page, e), at_row = __shfl_sync(0xffffffffu, offset, e);
+          const int at_page = __shfl_sync(0xffffffffu, good_page, e), at_row = __shfl_sync(0xffffffffu, t.offset, e);
           const char* k_src = k_head + at_page * p.kc.page_stride + at_row * p.kc.token_stride + k_lane;
           const char* v_src = v_head + at_page * p.vc.page_stride + at_row * p.vc.token_stride + v_lane;
 #pragma unroll
@@ -252,12 +283,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
             copy(e * 8 + r, k_src + r * p.kc.token_stride, v_src + r * p.vc.token_stride, at_page >= 0);
         }
       } else {
-        const int* table = p.page_table + static_cast<long long>(load.seq) * p.table_pages;
+        const int* table = p.page_table + static_cast<long long>(t.seq) * p.table_pages;
 #pragma unroll
         for (int r = 0; r < C::kKeys; r += kRowsPerCopy) {
           int at_page = -1, at_row = 0;
           if (r + lane_row < keys) {
-            const int key = key0 + r + lane_row, slot = fast_div(key, p.by_page);
+            const int key = t.key0 + r + lane_row, slot = fast_div(key, p.by_page);
             at_row = key - slot * static_cast<int>(p.by_page.d);
             at_page = __ldg(table + slot);
             if (static_cast<unsigned>(at_page) >= static_cast<unsigned>(p.pages)) {
@@ -270,34 +301,34 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
         }
       }
       if (++load_stage == kStages) load_stage = 0;
-      if (++load.step >= load.stop) advance(load);
-      look_up();
     }
     copies_commit();
   };
 
-  constexpr int kNT = DP / 8;                                  // 8-column tiles of the output
-  constexpr int kHalves = HALF ? 1 : 2;                        // rows lane / 4 and lane / 4 + 8
-  const int row0 = lane >> 2, col0 = (lane & 3) * 2;
+  constexpr int kNQ = HALF ? 1 : 2;                            // eights of query rows
+  constexpr int kMT = DP / 16;                                 // sixteens of the output's columns, and of the products' depth
+  const int col0 = (lane & 3) * 2, row0 = lane >> 2;
   int stage = 0;
-  uint32_t qf[DP / 16][4], q_next[DP / 16][2 * kHalves];
-  float o[kNT][4], m[2], sum[2];
+  uint32_t qf[kMT][kNQ][2], q_next[kMT][kNQ][2];
+  // o[i][q][c]: column 16 i + row0 (+ 8 where c > 1) of query 8 q + col0 + (c & 1); m and sum: of those two queries
+  float o[kMT][kNQ][4], m[kNQ][2], sum[kNQ][2];
   auto row_tile = [&](int item) { return item - head_of(item) * p.row_tiles; };
   auto rows_of = [&](int item) { return item < p.items ? min(kRows, p.group - row_tile(item) * kRows) : 0; };
   auto first_row = [&](int item) { return head_of(item) * p.group + row_tile(item) * kRows; };
-  // Queries as the products' left operand: registers [k][0] and [2] are row lane / 4, [1] and [3] row lane / 4 + 8.  The next
-  // item's are fetched while one is run.
+  // Queries as the first product's right operand; the next item's are fetched while one is run.
   auto fetch_q = [&](const Cursor& c) {
     if (c.stop < 0) return;
     const int item = item_of(c), rows = rows_of(item);
     const char* q = p.q.data + c.seq * p.q.token_stride + first_row(item) * p.q.head_stride;
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
+    for (int k = 0; k < kMT; ++k)
 #pragma unroll
-      for (int j = 0; j < 2 * kHalves; ++j) {
-        const int r = row0 + (HALF ? 0 : (j & 1) * 8), col = k * 16 + col0 + (HALF ? j : j >> 1) * 8;
-        q_next[k][j] = r >= rows || col >= p.dim ? 0u : __ldg(reinterpret_cast<const unsigned int*>(q + r * p.q.head_stride + col * 2));
-      }
+      for (int j = 0; j < kNQ; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = j * 8 + row0, col = k * 16 + e * 8 + col0;
+          q_next[k][j][e] = r >= rows || col >= p.dim ? 0u : __ldg(reinterpret_cast<const unsigned int*>(q + r * p.q.head_stride + col * 2));
+        }
   };
   auto row_of = [&](const Cursor& c, int item, int row) {
     return p.out + (static_cast<long long>(c.seq) * p.q_heads + first_row(item) + row) * p.dim * 2;
@@ -320,35 +351,39 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
     if (ahead == 0 && now.step >= now.stop) {
       if (running) {
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-          sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-        }
+        for (int q = 0; q < kNQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) sum[q][e] += __shfl_xor_sync(0xffffffffu, sum[q][e], d);
       }
       if (running && now.solo) {
-        const int item = item_of(now);
+        const int item = item_of(now), rows = rows_of(item);
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const int row = row0 + 8 * h;
-          if (row >= rows_of(item)) continue;
-          const float inv = sum[h] == 0.0f ? 0.0f : 1.0f / sum[h];
-          char* dst = row_of(now, item, row);
+        for (int q = 0; q < kNQ; ++q) {
+          const float inv0 = sum[q][0] == 0.0f ? 0.0f : 1.0f / sum[q][0], inv1 = sum[q][1] == 0.0f ? 0.0f : 1.0f / sum[q][1];
+          char* dst = row_of(now, item, q * 8 + row0);
 #pragma unroll
-          for (int n = 0; n < kNT; ++n)
-            if (n * 8 + col0 < p.dim)
-              *reinterpret_cast<uint32_t*>(dst + (n * 8 + col0) * 2) = pack2<T>(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
+          for (int i = 0; i < kMT; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {      // eight columns by eight queries, to a query a lane's four
+              const uint32_t v = transpose(pack2<T>(o[i][q][2 * e] * inv0, o[i][q][2 * e + 1] * inv1));
+              if (q * 8 + row0 < rows && i * 16 + e * 8 < p.dim) *reinterpret_cast<uint32_t*>(dst + (i * 16 + e * 8 + col0) * 2) = v;
+            }
         }
       } else if (running) {
         const int rows = rows_of(now.unit), all = steps_of(tiles_of(now.len));
         const bool enters = first_step > 0, leaves = now.stop < all;
-        PartialTile* part = p.partials + (run * 2 + (enters ? 0 : 1));
+        Partial* part = partials + (run * 2 + (enters ? 0 : 1));
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
+        for (int h = 0; h < kNQ; ++h) {
           team_sync();                         // what was there has been read
-          float* own = join + (member * 8 + row0) * C::kJoinRow;
+          float* own = join + (member * 8 + col0) * C::kJoinRow;
 #pragma unroll
-          for (int n = 0; n < kNT; ++n) *reinterpret_cast<float2*>(own + n * 8 + col0) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-          if ((lane & 3) == 0) *reinterpret_cast<float2*>(own + DP) = make_float2(m[h], sum[h]);
+          for (int i = 0; i < kMT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) own[(c & 1) * C::kJoinRow + i * 16 + (c >> 1) * 8 + row0] = o[i][h][c];
+          if (row0 < 2) *reinterpret_cast<float2*>(own + row0 * C::kJoinRow + DP) = make_float2(row0 ? m[h][1] : m[h][0], row0 ? sum[h][1] : sum[h][0]);
           team_sync();
 #pragma unroll 1
           for (int i = thread; i < 8 * DP / 4; i += kTeam) {
@@ -400,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
               if (col >= p.dim) continue;
               float top = kNegInf, row_sum = 0.0f;
               float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              constexpr int kBatch = 8;        // parts that are fetched at a time
+              constexpr int kBatch = 4;        // parts that are fetched at a time
 #pragma unroll 1
               for (int t0 = first; t0 <= last; t0 += kBatch) {
                 float pm[kBatch], ps[kBatch];
@@ -408,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
 #pragma unroll
                 for (int e = 0; e < kBatch; ++e) {
                   const int t = min(t0 + e, last);
-                  const PartialTile& x = p.partials[t * 2 + (t == first)];
+                  const Partial& x = partials[t * 2 + (t == first)];
                   pm[e] = t0 + e <= last ? __ldcg(&x.m[row]) : kNegInf;
                   ps[e] = __ldcg(&x.sum[row]);
                   po[e] = __ldcg(reinterpret_cast<const float4*>(&x.o[row][col]));
@@ -438,16 +473,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
       first_step = now.step;
       running = true;
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        qf[k][0] = q_next[k][0];
-        qf[k][1] = HALF ? 0u : q_next[k][HALF ? 0 : 1];
-        qf[k][2] = q_next[k][HALF ? 1 : 2];
-        qf[k][3] = HALF ? 0u : q_next[k][HALF ? 0 : 3];
-      }
+      for (int k = 0; k < kMT; ++k)
 #pragma unroll
-      for (int n = 0; n < kNT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-      m[0] = m[1] = kNegInf;
-      sum[0] = sum[1] = 0.0f;
+        for (int q = 0; q < kNQ; ++q) {
+          qf[k][q][0] = q_next[k][q][0];
+          qf[k][q][1] = q_next[k][q][1];
+          o[k][q][0] = o[k][q][1] = o[k][q][2] = o[k][q][3] = 0.0f;
+        }
+#pragma unroll
+      for (int q = 0; q < kNQ; ++q) {
+        m[q][0] = m[q][1] = kNegInf;
+        sum[q][0] = sum[q][1] = 0.0f;
+      }
       advance(next);
       fetch_q(next);
     }
@@ -463,104 +500,112 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const DecodeP
     if (++stage == kStages) stage = 0;
     ++now.step;
     if (keys <= 0) continue;
-    constexpr int kST = C::kKeys / 8;
-    float s[kST][4], odd[kST][4];              // products of even and odd sixteens of the head: two shorter chains
+    float s[kNQ][4], odd[kNQ][4];              // products of even and odd sixteens of the head: two shorter chains
 #pragma unroll
-    for (int n = 0; n < kST; ++n)
+    for (int q = 0; q < kNQ; ++q)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = odd[n][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) s[q][e] = odd[q][e] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
+    for (int k = 0; k < kMT; ++k) {
+      uint32_t a[4];
+      ldmatrix_x4(a, tile_k + (k >> 2) * C::kKeys * 128 + (lane & 15) * 128 + ((((k & 3) * 2 + (lane >> 4)) ^ (lane & 7)) << 4));
 #pragma unroll
-      for (int n = 0; n < kST / 2; ++n) {
-        uint32_t b[4];
-        const int row = n * 16 + (lane & 7) + (lane >> 4) * 8;
-        ldmatrix_x4(b, tile_k + (k >> 2) * C::kKeys * 128 + row * 128 + ((((k & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
-        mma_16816<T>(k & 1 ? odd[2 * n] : s[2 * n], qf[k], b[0], b[1]);
-        mma_16816<T>(k & 1 ? odd[2 * n + 1] : s[2 * n + 1], qf[k], b[2], b[3]);
-      }
-    float base[2], top[2];
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      top[h] = m[h];
-#pragma unroll
-      for (int n = 0; n < kST; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float& v = s[n][2 * h + j];
-          v = n * 8 + col0 + j < keys ? (v + odd[n][2 * h + j]) * p.scale_log2 : kNegInf;
-          top[h] = fmaxf(top[h], v);
-        }
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+      for (int q = 0; q < kNQ; ++q) mma_16816<T>(k & 1 ? odd[q] : s[q], a, qf[k][q][0], qf[k][q][1]);
     }
-    if (__any_sync(0xffffffffu, top[0] > m[0] || (!HALF && top[kHalves - 1] > m[kHalves - 1]))) {
+    float top[kNQ][2];
+    bool grown = false;
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const float keep = top[h] == kNegInf ? 1.0f : exp2_fast(m[h] - top[h]);
-        m[h] = top[h];
-        sum[h] *= keep;
+    for (int q = 0; q < kNQ; ++q) {
 #pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          o[n][2 * h] *= keep;
-          o[n][2 * h + 1] *= keep;
-        }
+      for (int e = 0; e < 4; ++e) s[q][e] = row0 + (e >> 1) * 8 < keys ? (s[q][e] + odd[q][e]) * p.scale_log2 : kNegInf;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[q][e] = fmaxf(s[q][e], s[q][2 + e]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top[q][e] = fmaxf(top[q][e], __shfl_xor_sync(0xffffffffu, top[q][e], d));
+        grown = grown || top[q][e] > m[q][e];
       }
     }
+    if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) base[h] = m[h] == kNegInf ? 0.0f : m[h];   // nothing but minus infinity yet: no difference
-    uint32_t pf[kST / 2][4];                                                     // of infinities
+      for (int q = 0; q < kNQ; ++q) {
+        float keep[2];
 #pragma unroll
-    for (int n = 0; n < kST; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h < kHalves) {
-          const float e0 = exp2_fast(s[n][2 * h] - base[h]), e1 = exp2_fast(s[n][2 * h + 1] - base[h]);
-          sum[h] += e0 + e1;
-          pf[n >> 1][(n & 1) * 2 + h] = pack2<T>(e0, e1);
-        } else {
-          pf[n >> 1][(n & 1) * 2 + h] = 0u;
+        for (int e = 0; e < 2; ++e) {
+          const float now_top = fmaxf(m[q][e], top[q][e]);
+          keep[e] = now_top == kNegInf ? 1.0f : exp2_fast(m[q][e] - now_top);
+          m[q][e] = now_top;
+          sum[q][e] *= keep[e];
         }
-      }
 #pragma unroll
-    for (int k = 0; k < kST / 2; ++k)
+        for (int i = 0; i < kMT; ++i)
 #pragma unroll
-      for (int n = 0; n < kNT / 2; ++n) {
-        uint32_t b[4];
-        const int row = k * 16 + (lane & 15), piece = n * 2 + (lane >> 4);
-        ldmatrix_x4_trans(b, tile_v + (n >> 2) * C::kKeys * 128 + row * 128 + (((piece & 7) ^ (lane & 7)) << 4));
-        mma_16816<T>(o[2 * n], pf[k], b[0], b[1]);
-        mma_16816<T>(o[2 * n + 1], pf[k], b[2], b[3]);
+          for (int c = 0; c < 4; ++c) o[i][q][c] *= keep[c & 1];
       }
+    }
+    uint32_t pf[kNQ][2];
+#pragma unroll
+    for (int q = 0; q < kNQ; ++q) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {            // (nothing but minus infinity so far: no difference of infinities)
+        w[e] = exp2_fast(s[q][e] - (m[q][e & 1] == kNegInf ? 0.0f : m[q][e & 1]));
+        sum[q][e & 1] += w[e];
+      }
+      pf[q][0] = transpose(pack2<T>(w[0], w[1]));
+      pf[q][1] = transpose(pack2<T>(w[2], w[3]));
+    }
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) {
+      uint32_t a[4];
+      ldmatrix_x4_trans(a, tile_v + (i >> 2) * C::kKeys * 128 + ((lane & 7) + (lane >> 4) * 8) * 128 +
+                               ((((i & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+#pragma unroll
+      for (int q = 0; q < kNQ; ++q) mma_16816<T>(o[i][q], a, pf[q][0], pf[q][1]);
+    }
     __syncwarp();              // the next copies overwrite this tile
   }
   copies_wait<0>();
 }
 
-template <typename T, int DP, bool HALF, bool EIGHTS>
-int launch_decode(const DecodeParams& p, int grid, cudaStream_t st) {
-  using C = Decode<T, DP, HALF, EIGHTS>;
+template <typename T, int DP, bool HALF, bool EIGHTS, bool WHOLE>
+int launch_decode(DecodeParams p, cudaStream_t st) {
+  using C = Decode<T, DP, HALF, EIGHTS, WHOLE>;
   static thread_local int configured_device = -1;
   int device = 0;
   MP_CUDA_TRY(cudaGetDevice(&device));
   if (configured_device != device) {
-    MP_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<T, DP, HALF, EIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    MP_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<T, DP, HALF, EIGHTS, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     configured_device = device;
   }
-  return launch_chained(paged_decode_kernel<T, DP, HALF, EIGHTS>, dim3(grid), dim3(kThreads), C::kSmem, st, p);
+  const long long items = static_cast<long long>(p.batch) * p.items;
+  // with an item to a team and more, warps take those of short sequences alone
+  p.solo_tiles = items >= kSmCount * C::kTeams ? kSoloTiles : 1;
+  // no more teams than there can be whole items and steps of what is cut; a block for every team of those
+  const long long step = C::kKeys * C::kTeamWarps, steps = (p.capacity + step - 1) / step;
+  const long long teams = items * (steps <= kWholeSteps ? 1 : steps);
+  const int grid = static_cast<int>(teams < kSmCount ? teams : kSmCount);
+  return launch_chained(paged_decode_kernel<T, DP, HALF, EIGHTS, WHOLE>, dim3(grid), dim3(C::kThreads), C::kSmem, st, p);
 }
 
+template <typename T, int DP, bool HALF, bool EIGHTS>
+int dispatch_teams(const DecodeParams& p, cudaStream_t st) {
+  // No more items than SMs: an SM's warps all go to one, which is then seldom cut (a sequence of 300 tokens and eight heads
+  // 8.7 us with teams of four warps).
+  return static_cast<long long>(p.batch) * p.items <= kSmCount ? launch_decode<T, DP, HALF, EIGHTS, true>(p, st)
+                                                               : launch_decode<T, DP, HALF, EIGHTS, false>(p, st);
+}
 template <typename T, int DP, bool EIGHTS>
-int dispatch_rows(const DecodeParams& p, int grid, cudaStream_t st) {
-  return p.group <= 8 ? launch_decode<T, DP, true, EIGHTS>(p, grid, st) : launch_decode<T, DP, false, EIGHTS>(p, grid, st);
+int dispatch_rows(const DecodeParams& p, cudaStream_t st) {
+  return p.group <= 8 ? dispatch_teams<T, DP, true, EIGHTS>(p, st) : dispatch_teams<T, DP, false, EIGHTS>(p, st);
 }
 template <typename T, int DP>
-int dispatch_pages(const DecodeParams& p, int grid, cudaStream_t st) {
-  return p.by_page.d % 8 == 0 ? dispatch_rows<T, DP, true>(p, grid, st) : dispatch_rows<T, DP, false>(p, grid, st);
+int dispatch_pages(const DecodeParams& p, cudaStream_t st) {
+  return p.by_page.d % 8 == 0 ? dispatch_rows<T, DP, true>(p, st) : dispatch_rows<T, DP, false>(p, st);
 }
 template <typename T>
-int dispatch_decode(const DecodeParams& p, int grid, cudaStream_t st) {
-  return p.dim <= 64 ? dispatch_pages<T, 64>(p, grid, st) : dispatch_pages<T, 128>(p, grid, st);
+int dispatch_decode(const DecodeParams& p, cudaStream_t st) {
+  return p.dim <= 64 ? dispatch_pages<T, 64>(p, st) : dispatch_pages<T, 128>(p, st);
 }
 
 }  // namespace
@@ -584,7 +629,7 @@ extern "C" int mp_paged_attention_decode(int dtype, const mp_head_rows* q, int B
   p.seq_lens = static_cast<const int*>(seq_lens_i32);
   p.out = static_cast<char*>(out);
   p.counters = static_cast<int*>(workspace);
-  p.partials = reinterpret_cast<PartialTile*>(static_cast<char*>(workspace) + kCounterBytes);
+  p.partials = static_cast<char*>(workspace) + kCounterBytes;
   p.index_word = index_word;
   p.batch = B;
   p.q_heads = Hq;
@@ -599,13 +644,6 @@ extern "C" int mp_paged_attention_decode(int dtype, const mp_head_rows* q, int B
   p.capacity = static_cast<int>(room < 0x7fffff00LL ? room : 0x7fffff00LL);
   p.scale_log2 = scale * attn::kLog2e;
   p.by_page = make_fast_div(cache->page_size);
-  const int keys = D <= 64 ? Decode<__half, 64, true, true>::kKeys : Decode<__half, 128, true, true>::kKeys;
-  // with four items to a team and more, warps take those of short sequences alone
-  p.solo_tiles = static_cast<long long>(B) * p.items >= 4 * kMaxTeams ? kSoloTiles : 1;
-  // no more teams than there can be whole items and steps of what is cut
-  const long long steps = (p.capacity + keys * kTeamWarps - 1LL) / (keys * kTeamWarps);
-  const long long teams = static_cast<long long>(B) * p.items * (steps <= kWholeSteps ? 1 : steps);
-  const int grid = static_cast<int>(teams < kSmCount ? teams : kSmCount);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == 0 ? dispatch_decode<__half>(p, grid, st) : dispatch_decode<__nv_bfloat16>(p, grid, st);
+  return dtype == 0 ? dispatch_decode<__half>(p, st) : dispatch_decode<__nv_bfloat16>(p, st);
 }
