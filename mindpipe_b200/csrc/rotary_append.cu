@@ -31,6 +31,7 @@ struct AppendParams {
 
 // How a head's pairs lie: halves whose 16-byte pieces correspond; neighbours; halves that begin inside a piece.
 enum { kHalves = 0, kNeighbours = 1, kOddHalves = 2 };
+constexpr int kMostThreads = 256;
 
 __device__ __forceinline__ uint4 load16(const char* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
@@ -54,8 +55,7 @@ __device__ __forceinline__ void rotate_pieces(uint4& a, uint4& b, const float* c
 
 // The piece at column `col` of a head whose pairs are neighbours, or whose halves do not begin at a piece.
 template <typename T, int MODE>
-__device__ __forceinline__ uint4 rotate_piece(const char* head, int col, int rotated, const float* row) {
-  uint4 raw = load16(head + col * 2);
+__device__ __forceinline__ uint4 rotate_piece(uint4 raw, const char* head, int col, int rotated, const float* row) {
   uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
   const int half = rotated / 2;
 #pragma unroll
@@ -84,73 +84,54 @@ __device__ __forceinline__ uint4 rotate_piece(const char* head, int col, int rot
   return raw;
 }
 
-// Block (t, y): pieces of work 256 y .. of token t.  `items`: those of the q heads, the k heads, then the pieces of v.
+// Block (t, y): pieces of work blockDim y .. of token t: those of the q heads, the k heads, then the pieces of v.  The values
+// are asked for before anything that hangs on the token's position and slot (one wait for memory, not two in a row: a prompt
+// of 8192 tokens and 64 heads 68.6 us before).
 template <typename T, int MODE>
-__global__ void __launch_bounds__(256) rotary_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kMostThreads, 2048 / kMostThreads) rotary_append_kernel(const AppendParams p) {
   chain_wait();
   chain_release();
-  const int t = blockIdx.x, item = blockIdx.y * 256 + threadIdx.x;
+  const int t = blockIdx.x, item = blockIdx.y * blockDim.x + threadIdx.x;
   if (item >= p.items) return;
-  int pos = __ldg(p.positions + t);
-  const int slot = __ldg(p.slots + t);
-  const bool bad_pos = pos < 0 || pos >= p.max_positions;
-  bool stored = slot >= 0;
-  if (bad_pos) pos = 0;
-  if ((stored && bad_pos) || slot >= p.slot_count) {
-    if (p.index_word && item == 0) *p.index_word = kBadIndex;
-    stored = false;
-  }
-  const int page = fast_div(max(slot, 0), p.by_page), offset = max(slot, 0) - page * static_cast<int>(p.by_page.d);
-  const long long t64 = t;
-
+  const int pos_there = __ldg(p.positions + t), slot = __ldg(p.slots + t);
   const int rotated_items = (p.q_heads + p.kv_heads) * p.per_head;
-  if (item >= rotated_items) {           // values are copied
-    if (!stored) return;
-    const int i = item - rotated_items, head = fast_div(i, p.by_pieces), piece = i - head * static_cast<int>(p.by_pieces.d);
-    const uint4 x = load16(p.v.data + t64 * p.v.token_stride + head * p.v.head_stride + piece * 16);
-    *reinterpret_cast<uint4*>(p.vc.data + page * p.vc.page_stride + head * p.vc.head_stride + offset * p.vc.token_stride +
-                              piece * 16) = x;
-    return;
-  }
-  const int head = fast_div(item, p.by_per_head), piece = item - head * p.per_head;
-  const bool is_q = head < p.q_heads;
-  const int kv = head - p.q_heads;
-  const char* src = is_q ? p.q.data + t64 * p.q.token_stride + head * p.q.head_stride
-                         : p.k.data + t64 * p.k.token_stride + kv * p.k.head_stride;
-  char* dst = is_q ? p.q_out + (t64 * p.q_heads + head) * p.head_bytes
-                   : p.k_out ? p.k_out + (t64 * p.kv_heads + kv) * p.head_bytes : nullptr;
-  char* cached = is_q || !stored ? nullptr
-                                 : p.kc.data + page * p.kc.page_stride + kv * p.kc.head_stride + offset * p.kc.token_stride;
-  const float* row = p.table + static_cast<long long>(pos) * p.rotated;
-  if (MODE == kHalves) {
-    const int pairs = p.rotated / 16;
-    if (piece < pairs) {
-      uint4 a = load16(src + piece * 16), b = load16(src + (piece + pairs) * 16);
-      rotate_pieces<T>(a, b, row + piece * 8, row + p.rotated / 2 + piece * 8);
-      if (dst) {
-        *reinterpret_cast<uint4*>(dst + piece * 16) = a;
-        *reinterpret_cast<uint4*>(dst + (piece + pairs) * 16) = b;
-      }
-      if (cached) {
-        *reinterpret_cast<uint4*>(cached + piece * 16) = a;
-        *reinterpret_cast<uint4*>(cached + (piece + pairs) * 16) = b;
-      }
-      return;
-    }
-    const int at = (piece + pairs) * 16;         // behind the rotated part
-    const uint4 x = load16(src + at);
-    if (dst) *reinterpret_cast<uint4*>(dst + at) = x;
-    if (cached) *reinterpret_cast<uint4*>(cached + at) = x;
-  } else {
-    const uint4 x = rotate_piece<T, MODE>(src, piece * 8, p.rotated, row);
-    if (dst) *reinterpret_cast<uint4*>(dst + piece * 16) = x;
-    if (cached) *reinterpret_cast<uint4*>(cached + piece * 16) = x;
+  const bool is_v = item >= rotated_items;
+  const int i = is_v ? item - rotated_items : item;
+  const int head = fast_div(i, is_v ? p.by_pieces : p.by_per_head), piece = i - head * (is_v ? static_cast<int>(p.by_pieces.d) : p.per_head);
+  const bool is_q = !is_v && head < p.q_heads;
+  const int own = is_q || is_v ? head : head - p.q_heads;
+  const HeadRows& rows = is_v ? p.v : is_q ? p.q : p.k;
+  const char* src = rows.data + static_cast<long long>(t) * rows.token_stride + own * rows.head_stride;
+  const int pairs = p.rotated / 16;
+  const bool turns = MODE == kHalves && !is_v && piece < pairs;             // both halves of eight pairs
+  const int at = (MODE == kHalves && !is_v && piece >= pairs ? piece + pairs : piece) * 16;
+  uint4 a = load16(src + at), b = make_uint4(0, 0, 0, 0);
+  if (turns) b = load16(src + at + pairs * 16);
+
+  const bool bad_pos = static_cast<unsigned>(pos_there) >= static_cast<unsigned>(p.max_positions);
+  const bool bad = (slot >= 0 && bad_pos) || slot >= p.slot_count;
+  if (bad && p.index_word && item == 0) *p.index_word = kBadIndex;
+  const float* row = p.table + static_cast<long long>(bad_pos ? 0 : pos_there) * p.rotated;
+  if (turns) rotate_pieces<T>(a, b, row + piece * 8, row + p.rotated / 2 + piece * 8);
+  else if (MODE != kHalves && !is_v) a = rotate_piece<T, MODE>(a, src, piece * 8, p.rotated, row);
+  auto put = [&](char* dst) {
+    *reinterpret_cast<uint4*>(dst + at) = a;
+    if (turns) *reinterpret_cast<uint4*>(dst + at + pairs * 16) = b;
+  };
+  char* out = is_v ? nullptr : is_q ? p.q_out : p.k_out;
+  if (out) put(out + (static_cast<long long>(t) * (is_q ? p.q_heads : p.kv_heads) + own) * p.head_bytes);
+  if (!is_q && slot >= 0 && !bad) {
+    const CacheSide& side = is_v ? p.vc : p.kc;
+    const int page = fast_div(slot, p.by_page), offset = slot - page * static_cast<int>(p.by_page.d);
+    put(side.data + page * side.page_stride + own * side.head_stride + offset * side.token_stride);
   }
 }
 
 template <typename T>
 int launch_append(const AppendParams& p, int mode, int tokens, cudaStream_t st) {
-  const dim3 grid(tokens, (p.items + 255) / 256), block(256);
+  // blocks of even size, so that few threads are idle
+  const int blocks = (p.items + kMostThreads - 1) / kMostThreads, threads = ((p.items + blocks - 1) / blocks + 31) / 32 * 32;
+  const dim3 grid(tokens, blocks), block(threads);
   switch (mode) {
     case kHalves: return launch_chained(rotary_append_kernel<T, kHalves>, grid, block, 0, st, p);
     case kNeighbours: return launch_chained(rotary_append_kernel<T, kNeighbours>, grid, block, 0, st, p);
