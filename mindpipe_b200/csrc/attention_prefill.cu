@@ -29,9 +29,9 @@ using namespace tc;
 
 constexpr int kTile = 128;                     // query rows of a tile and keys of a step
 // Four warps of copies, products, planning and nothing, and two groups of four.  Registers: the block starts with 168 a
-// thread, 64512 in all; the first four warps give back what the others take, 128 x 56 + 256 x 224 = 64512.
+// thread, 64512 in all; the first four warps give back what the others take, 128 x 72 + 256 x 216 = 64512.
 constexpr int kWarps = 12, kThreads = 32 * kWarps;
-constexpr int kFewRegisters = 56, kManyRegisters = 224;
+constexpr int kFewRegisters = 72, kManyRegisters = 216;
 constexpr int kTmemCols = 512;
 constexpr float kGrowth = 8.0f;                // log2 of how far weights may exceed 1
 constexpr int kAhead = 4;                      // items that the planning warp is ahead
@@ -41,9 +41,10 @@ template <int DP>
 struct Prefill {
   static constexpr int kBoxes = DP / 64;                       // copies of 64 columns
   static constexpr int kTileBytes = kTile * DP * 2;
-  static constexpr int kStages = DP == 64 ? 8 : 5;
+  static constexpr int kStages = 4;
   static constexpr int kBarBytes = 512;
-  static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + kBarBytes + 1024;
+  static constexpr int kOutBytes = 8 * 32 * 128;               // 32 rows of 64 columns for each of eight warps
+  static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + kOutBytes + kBarBytes + 1024;
 };
 
 struct MapOrder {
@@ -146,54 +147,46 @@ __device__ __forceinline__ float exp2_ordered(float x) {
   return y;
 }
 
-// Weights 2^(s scale - ref) of 16 scores, their sum added to `sum` and the weights rounded to eight words.  Two of the eight
-// pairs are computed by multiplications while the exponential unit has the others: x = n + f with n the nearest integer, 2^f
+// Weights 2^(s scale - ref) of 16 scores, their sum added to `sum` and the weights rounded to eight words.  One of the eight
+// pairs is computed by multiplications while the exponential unit has the others: x = n + f with n the nearest integer, 2^f
 // by a polynomial of degree 5 (minimax on [-1/2, 1/2], found by exchange; relative error 2^-23.6), n added to the exponent.
 // x is at most about 2^7; below -127 it counts as -127, which gives 0.  (A NaN does not come through there: see the maximum.)
-// The unit takes 16 values a clock and SM; with one warp on a scheduler 128 scores take 984 clocks in this order and 1650
-// as the compiler orders a plain loop, with two 1704 together and 2100 without the multiplications.
+// The unit takes 16 values a clock and SM, 1024 clocks for a tile.  In this order, by hand, the instructions of a warp that
+// is alone on its scheduler keep it busy; as the compiler orders a plain loop they took 1650.  2048 tokens of 32 heads with
+// none, one, two, three of eight by multiplications: 49.2, 48.5, 49.3, 52.9 us.
 // between(m), m = 0..6: what else can be done meanwhile.
 template <typename T, typename F>
 __device__ __forceinline__ void exp2_batch(const uint32_t* s, F2 scale, F2 minus_ref, F2& sum, uint32_t* packed, F between) {
   constexpr float kMagic = 12582912.0f;        // 1.5 * 2^23: added, the sum's low bits are the nearest integer
   constexpr float kC[6] = {1.3276472454890609e-3f, 9.675540961325169e-3f, 5.550713092088699e-2f,
                            0.24022120237350464f, 0.6931469440460205f, 1.0000001192092896f};
-  F2 x[8], t[2], f[2], r[2];
+  F2 x[8], t, f, r;
   float v[16];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = fma2(f2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale, minus_ref);
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
+  {
     float a, b;
-    split(x[6 + e], a, b);
-    x[6 + e] = f2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
-    t[e] = add2(x[6 + e], f2(kMagic, kMagic));
+    split(x[7], a, b);
+    x[7] = f2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
+    t = add2(x[7], f2(kMagic, kMagic));
   }
 #pragma unroll
   for (int m = 0; m < 7; ++m) {
-    if (m < 6) {
-      float a, b;
-      split(x[m], a, b);
-      v[2 * m] = exp2_ordered(a);
-      v[2 * m + 1] = exp2_ordered(b);
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (m == 0) f[e] = fma2(t[e], f2(-1.0f, -1.0f), f2(kMagic, kMagic));
-      if (m == 1) f[e] = add2(x[6 + e], f[e]);
-      if (m == 2) r[e] = fma2(f2(kC[0], kC[0]), f[e], f2(kC[1], kC[1]));
-      if (m > 2) r[e] = fma2(r[e], f[e], f2(kC[m - 1], kC[m - 1]));
-    }
+    float a, b;
+    split(x[m], a, b);
+    v[2 * m] = exp2_ordered(a);
+    v[2 * m + 1] = exp2_ordered(b);
+    if (m == 0) f = fma2(t, f2(-1.0f, -1.0f), f2(kMagic, kMagic));
+    if (m == 1) f = add2(x[7], f);
+    if (m == 2) r = fma2(f2(kC[0], kC[0]), f, f2(kC[1], kC[1]));
+    if (m > 2) r = fma2(r, f, f2(kC[m - 1], kC[m - 1]));
     between(m);
   }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    float a, b, t0, t1;
-    split(r[e], a, b);
-    split(t[e], t0, t1);
-    v[12 + 2 * e] = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
-    v[13 + 2 * e] = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
-  }
+  float a, b, t0, t1;
+  split(r, a, b);
+  split(t, t0, t1);
+  v[14] = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
+  v[15] = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     sum = add2(sum, f2(v[2 * e], v[2 * e + 1]));
@@ -319,7 +312,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   using C = Prefill<DP>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (2 + C::kStages) * C::kTileBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (2 + C::kStages) * C::kTileBytes + C::kOutBytes);
   const uint32_t q_tile = smem_u32(smem), ring = q_tile + 2 * C::kTileBytes;
   const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * C::kStages, q_full = kv_empty + 8 * C::kStages,
                  q_empty = q_full + 16, s_full = q_empty + 16, p_ready = s_full + 16 /* [tile][half of the keys] */,
@@ -729,24 +722,36 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       if (!wait_all(o_done + 8 * i, o_phase ^ 1)) { ok = false; break; }
       tcgen05_fence_after();
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int at = row_begin + row;
-      char* dst = p.out + ((static_cast<long long>(seq_begin) + at) * p.q_heads + head) * p.dim * 2;
+      // 64 columns at a time through shared memory, so that a warp's stores are whole lines (a row to a thread took 3000 clocks
+      // of an item's end)
+      const uint32_t staged = ring + C::kStages * C::kTileBytes + ((warp - 4) * 32) * 128;
+      const int first_row = row_begin + quarter * 32;
+      char* dst = p.out + ((static_cast<long long>(seq_begin) + first_row) * p.q_heads + head) * p.dim * 2;
 #pragma unroll 1
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32(o_tmem + 32 * c, o);
+      for (int c = 0; c < C::kBoxes; ++c) {
+        uint32_t o[2][32];
+        tmem_ld_32x32(o_tmem + 64 * c, o[0]);
+        tmem_ld_32x32(o_tmem + 64 * c + 32, o[1]);
         tmem_ld_wait();
-        if (at < len) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t word[4];
+        for (int e = 0; e < 8; ++e) {
+          uint32_t word[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              word[x] = pack2<T>(__uint_as_float(o[e * 8 + 2 * x]) * inv, __uint_as_float(o[e * 8 + 2 * x + 1]) * inv);
-            if (c * 32 + e * 8 < p.dim)
-              *reinterpret_cast<uint4*>(dst + (c * 32 + e * 8) * 2) = make_uint4(word[0], word[1], word[2], word[3]);
-          }
+          for (int x = 0; x < 4; ++x)
+            word[x] = pack2<T>(__uint_as_float(o[e >> 2][(e & 3) * 8 + 2 * x]) * inv, __uint_as_float(o[e >> 2][(e & 3) * 8 + 2 * x + 1]) * inv);
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(staged + lane * 128 + ((e ^ (lane & 7)) << 4)), "r"(word[0]), "r"(word[1]),
+                       "r"(word[2]), "r"(word[3]) : "memory");
         }
+        __syncwarp();
+        const int piece = lane & 7;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int r = e * 4 + (lane >> 3);
+          const uint4 v = lds16(staged + r * 128 + ((piece ^ (r & 7)) << 4));
+          if (first_row + r < len && c * 64 + piece * 8 < p.dim)
+            *reinterpret_cast<uint4*>(dst + (static_cast<long long>(r) * p.q_heads * p.dim + c * 64 + piece * 8) * 2) = v;
+        }
+        __syncwarp();
       }
       tcgen05_fence_before();
     }
