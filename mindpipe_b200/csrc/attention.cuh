@@ -64,15 +64,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Rows of DP 16-bit values in shared memory, in pieces of 16 bytes.  The pieces of a row are exchanged so that eight
-// consecutive rows have the same piece in eight different groups of banks (what ldmatrix reads at once).
-template <int DP>
-__device__ __forceinline__ uint32_t piece_at(int row, int piece) {
-  static_assert(DP % 32 == 0, "");
-  const int sw = DP % 64 == 0 ? (row & 7) : ((row >> 1) & 3);
-  return static_cast<uint32_t>(row * (DP * 2) + ((piece ^ sw) << 4));
-}
-
 }  // namespace attn
 
 // A [rows, heads, D] operand with strides in values; the last dimension is dense.

@@ -12,8 +12,8 @@
 //   warps 4-7 and 8-11, one group to a tile: a thread has one row; it takes S from tensor memory, the row's maximum, the
 //            exponentials, and leaves P, rounded, where S was
 //
-// The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights stay below
-// that in either type, the sum is in fp32), so most tiles leave O alone.  Bounds: for heads of 128 values a tile's two
+// The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights stay in
+// either type's range, the sum is in fp32), so most tiles leave O alone.  Bounds: for heads of 128 values a tile's two
 // products take the tensor cores 1024 clocks and its 16384 exponentials as many.
 //
 // What a row may not attend to must not reach it, whatever it holds: scores are replaced where masked, but 0 x NaN is NaN in
@@ -33,7 +33,10 @@ constexpr int kTile = 128;                     // query rows of a tile and keys 
 constexpr int kWarps = 12, kThreads = 32 * kWarps;
 constexpr int kFewRegisters = 72, kManyRegisters = 216;
 constexpr int kTmemCols = 512;
-constexpr float kGrowth = 8.0f;                // log2 of how far weights may exceed 1
+constexpr float kGrowth = 8.0f;                // log2 of how far a row's maximum may grow before it is taken
+// Weights are 2^(s - m + lift), rounded to the type before the product with V: below 2^15 in fp16, where many weights beneath
+// the type's 24 bits below 1 would be lost together.
+template <typename T> constexpr float kLift = __is_same(T, __half) ? 15.0f - kGrowth : 0.0f;
 constexpr int kAhead = 4;                      // items that the planning warp is ahead
 constexpr int kSortedBatch = 256;              // sequences whose tiles are taken longest first
 
@@ -607,7 +610,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         uint32_t packed[32];
         for (bool again = j == 0;; again = true) {
           const float ref = m == kNegInf ? 0.0f : m;
-          minus_ref = f2(-ref, -ref);
+          minus_ref = f2(kLift<T> - ref, kLift<T> - ref);
           part = 0;
 #pragma unroll
           for (int b = 0; b < 4; ++b)

@@ -12,8 +12,9 @@
 // one copies while the other joins.  A warp is a stream of its own: it copies its tiles of keys and values to its part of
 // shared memory (cp.async: a lane's 16 bytes go where ldmatrix finds them without conflicts, and what is not to be read
 // becomes zero; TMA's boxes of 128 bytes a row came at 6.0 TB/s where these come at 6.4), several ahead, also across the
-// ends of sequences, and it keeps its own maximum, sum and output until the team joins at the item's end.  The warps of a team take neighbouring tiles (with a run of tiles for
-// each warp, and no joins but at the run's ends, the cache's rate fell from 6.4 to 5.7 TB/s).  Where an item spans teams they
+// ends of sequences, and it keeps its own maximum, sum and output until the team joins at the item's end.  The warps of a
+// team take neighbouring tiles (with a run of tiles for each warp, and no joins but at the run's ends, the cache's rate fell
+// from 6.4 to 5.7 TB/s).  Where an item spans teams they
 // leave (m, sum, o) in the workspace, and the one that arrives last joins them in the teams' order, so results do not depend
 // on which one that was.  Of short sequences, where there are many, a team's warps take an item each, four heads at a time, and
 // need not join (301 sequences of 1 to 700 tokens and five heads: 25 us with four warps to every item).
@@ -31,6 +32,9 @@ constexpr int kStages = 3;
 constexpr int kRows = 16;                                     // query heads per tile
 constexpr int kItemCost = 2;           // what an item costs beside its steps, in steps
 constexpr int kWholeSteps = 4;         // steps up to which an item is not cut: a join of teams takes 2-3 us
+// Weights are 2^(s - m + lift), rounded to the type before the product with V.  fp16 has no more than 24 bits below 1, and many
+// weights beneath those would be lost together; multiplied by 2^15 they keep all their bits down to 2^-29.
+template <typename T> constexpr float kLift = __is_same(T, __half) ? 15.0f : 0.0f;
 constexpr int kSoloTiles = 8;          // tiles of a sequence up to which a warp takes an item alone, if there are many items
 
 // A team's two parts of items that it shares: the one it begins within (0) and the one it ends within (1).
@@ -140,9 +144,8 @@ __global__ void __launch_bounds__(Decode<T, DP, HALF, EIGHTS, WHOLE>::kThreads, 
 #pragma unroll 1
   for (int s = threadIdx.x * slice, n = 0; n < slice && s < p.batch; ++s, ++n) {
     const int tiles = tiles_of(length_of(s));
-    const unsigned cost = static_cast<unsigned>(steps_of(tiles) + kItemCost) * units_of(tiles);
-    sum_cost += cost;
-    about += static_cast<float>(cost);
+    sum_cost += static_cast<unsigned>(steps_of(tiles) + kItemCost) * units_of(tiles);
+    about += static_cast<float>(steps_of(tiles) + kItemCost) * static_cast<float>(units_of(tiles));
   }
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(Decode<T, DP, HALF, EIGHTS, WHOLE>::kThreads, 
   }
   s_scan[threadIdx.x] = sum_cost;
   if (lane == 31) s_warp[warp] = sum_cost;
-  // sums have 31 bits: a slice of 2^23 steps, 272 GB of keys and values, is refused
+  // sums have 32 bits: a slice of 2^23 steps -- half a billion tokens -- is refused (with pages that are named many times)
   if (__syncthreads_or(about > 8388607.0f)) {
     if (p.index_word) *p.index_word = kBadIndex;
     return;
@@ -549,7 +552,7 @@ __global__ void __launch_bounds__(Decode<T, DP, HALF, EIGHTS, WHOLE>::kThreads, 
       float w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {            // (nothing but minus infinity so far: no difference of infinities)
-        w[e] = exp2_fast(s[q][e] - (m[q][e & 1] == kNegInf ? 0.0f : m[q][e & 1]));
+        w[e] = exp2_fast(s[q][e] - (m[q][e & 1] == kNegInf ? 0.0f : m[q][e & 1] - kLift<T>));
         sum[q][e & 1] += w[e];
       }
       pf[q][0] = transpose(pack2<T>(w[0], w[1]));
@@ -622,7 +625,7 @@ extern "C" int mp_paged_attention_decode(int dtype, const mp_head_rows* q, int B
   int rc;
   if ((rc = check_head_rows(q, D, &p.q)) || (rc = check_cache(cache, D, &p.kc, &p.vc))) return rc;
   if (!page_table_i32 || !seq_lens_i32 || !out || B <= 0 || Hq <= 0 || table_pages <= 0) return MP_ERR_INVALID_ARG;
-  if ((dtype != 0 && dtype != 1) || Hq % cache->kv_heads || Hq > 65535) return MP_ERR_UNSUPPORTED;
+  if ((dtype != 0 && dtype != 1) || Hq % cache->kv_heads || Hq > 65535 || B > (1 << 30)) return MP_ERR_UNSUPPORTED;
   if (!aligned(out, 16) || !aligned(workspace, 16)) return MP_ERR_ALIGNMENT;
   if (!workspace || workspace_bytes < kWorkspaceBytes) return MP_ERR_WORKSPACE;
   p.page_table = static_cast<const int*>(page_table_i32);
