@@ -157,11 +157,16 @@ class PagedKVCache:
     def reserve(self, batch: int, longest: int) -> Step:
         """An empty step of ``batch`` sequences of up to ``longest`` tokens for :meth:`next_token`'s ``into``: no token of it
         is stored and its rows attend to nothing until it is filled."""
+        if batch < 1 or longest < 1:
+            raise ValueError("a step has at least one sequence, of at least one token")
         width = -(-longest // self.page_size)
         return Step([], self._tensor([0] * batch), self._tensor([-1] * batch), page_table=self._tensor([[-1] * width] * batch),
                     seq_lens=self._tensor([0] * batch))
 
     def free(self, sequences) -> None:
+        sequences = list(sequences)
+        if len(set(sequences)) != len(sequences) or not all(s in self._pages for s in sequences):
+            raise KeyError(f"not all of {sequences} are sequences of this cache, each once")
         for s in sequences:
             self._free.extend(reversed(self._pages.pop(s)))
             del self._length[s]
@@ -198,6 +203,8 @@ class PagedSelfAttention(nn.Module):
             width = getattr(self, name).out_features
             if width != cache.pool.shape[3] * self.head_dim:
                 raise ValueError(f"{name} gives {width} values, the cache holds {cache.pool.shape[3]} heads of {self.head_dim}")
+        if self.o_proj.in_features != self.q_proj.out_features:
+            raise ValueError(f"q_proj gives {self.q_proj.out_features} values, o_proj takes {self.o_proj.in_features}")
         if self.q_proj.out_features % (cache.pool.shape[3] * self.head_dim):
             raise ValueError("the query heads are not a multiple of the key heads")
         self.layer_idx, self.scale, self.interleaved = layer, scale, interleaved

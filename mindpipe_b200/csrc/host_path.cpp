@@ -628,7 +628,7 @@ long long stride_of(const at::Tensor& t, int i) { return t.size(i) <= 1 ? 0 : t.
 mp_head_rows head_rows(const at::Tensor& t) { return mp_head_rows{t.data_ptr(), stride_of(t, 0), stride_of(t, 1)}; }
 
 // the cache as k_cache and v_cache [pages, kv heads, page size, D]
-bool cache_arg(AttentionCall& call, PyObject* ko, PyObject* vo, const at::Tensor** k, mp_paged_cache* c) {
+bool cache_arg(AttentionCall& call, PyObject* ko, PyObject* vo, const at::Tensor** k, const at::Tensor** v_out, mp_paged_cache* c) {
   const at::Tensor* v;
   if (!call.values(ko, "k_cache", k, 4) || !call.values(vo, "v_cache", &v, 4)) return false;
   if ((*k)->sizes() != v->sizes()) return call.fail("k_cache and v_cache shapes differ");
@@ -636,6 +636,7 @@ bool cache_arg(AttentionCall& call, PyObject* ko, PyObject* vo, const at::Tensor
   *c = mp_paged_cache{(*k)->data_ptr(), v->data_ptr(), static_cast<int>((*k)->size(0)), static_cast<int>((*k)->size(1)),
                       static_cast<int>((*k)->size(2)), stride_of(**k, 0), stride_of(**k, 1), stride_of(**k, 2),
                       stride_of(*v, 0), stride_of(*v, 1), stride_of(*v, 2)};
+  *v_out = v;
   return true;
 }
 
@@ -654,6 +655,27 @@ bool output_arg(AttentionCall& call, PyObject* o, const at::Tensor& like, at::Te
   return true;
 }
 
+// The bytes from a tensor's first value to its last one.
+std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += std::max<int64_t>(t.size(i) - 1, 0) * t.stride(i);
+  const uintptr_t first = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {first, first + static_cast<uintptr_t>(last + 1) * t.element_size()};
+}
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  const auto x = span_of(a), y = span_of(b);
+  return x.second <= y.first || y.second <= x.first;
+}
+// Results may replace the queries (a tile's or an item's are read before its result is written, and by nobody else), but be
+// nothing else that a call reads.
+bool output_apart(AttentionCall& call, const at::Tensor& out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
+  const bool same = out.data_ptr() == q.data_ptr() && q.is_contiguous();
+  if ((!same && !apart(out, q)) || !apart(out, k) || !apart(out, v))
+    return call.fail("out overlaps an operand (it may be q itself, where that is contiguous)");
+  return true;
+}
+
 // (q_out, k_out or None), or the error status as an int
 PyObject* rotary_append(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
@@ -662,12 +684,16 @@ PyObject* rotary_append(PyObject*, PyObject* args) {
   unsigned long long word;
   if (!PyArg_ParseTuple(args, "OOOOOOOOppK", &qo, &ko, &vo, &to, &po, &so, &kco, &vco, &interleaved, &want_k, &word)) return nullptr;
   AttentionCall call;
-  const at::Tensor *q, *k, *v, *table, *pos, *slots, *kc;
+  const at::Tensor *q, *k, *v, *table, *pos, *slots, *kc, *vc;
   mp_paged_cache cache;
   if (!call.values(qo, "q", &q, 3, true) || !call.values(ko, "k", &k, 3) || !call.values(vo, "v", &v, 3) ||
       !call.dense(to, "cos_sin", &table, 2, at::kFloat) || !call.dense(po, "positions", &pos, 1, at::kInt) ||
-      !call.dense(so, "slots", &slots, 1, at::kInt) || !cache_arg(call, kco, vco, &kc, &cache))
+      !call.dense(so, "slots", &slots, 1, at::kInt) || !cache_arg(call, kco, vco, &kc, &vc, &cache))
     return nullptr;
+  if (kc->data_ptr() == vc->data_ptr()) return call.fail("k_cache and v_cache are the same memory"), nullptr;
+  for (int i = 0; i < 4; ++i)
+    if ((kc->size(i) > 1 && kc->stride(i) == 0) || (vc->size(i) > 1 && vc->stride(i) == 0))
+      return call.fail("the cache's entries share memory (an expanded tensor)"), nullptr;
   const int64_t t = q->size(0), d = q->size(2), rotated = table->size(1);
   if (k->sizes() != v->sizes() || k->size(0) != t || k->size(2) != d || k->size(1) != cache.kv_heads || kc->size(3) != d)
     return call.fail("q, k, v and cache shapes are inconsistent"), nullptr;
@@ -698,9 +724,9 @@ PyObject* paged_decode(PyObject*, PyObject* args) {
   unsigned long long word;
   if (!PyArg_ParseTuple(args, "OOOOOOOK", &qo, &kco, &vco, &to, &lo, &scale_o, &oo, &word)) return nullptr;
   AttentionCall call;
-  const at::Tensor *q, *kc, *table, *lens;
+  const at::Tensor *q, *kc, *vc, *table, *lens;
   mp_paged_cache cache;
-  if (!call.values(qo, "q", &q, 3, true) || !cache_arg(call, kco, vco, &kc, &cache) ||
+  if (!call.values(qo, "q", &q, 3, true) || !cache_arg(call, kco, vco, &kc, &vc, &cache) ||
       !call.dense(to, "page_table", &table, 2, at::kInt) || !call.dense(lo, "seq_lens", &lens, 1, at::kInt))
     return nullptr;
   const int64_t b = q->size(0), h = q->size(1), d = q->size(2);
@@ -711,7 +737,7 @@ PyObject* paged_decode(PyObject*, PyObject* args) {
   if (PyErr_Occurred()) return nullptr;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(call.device));
   at::Tensor out;
-  if (!output_arg(call, oo, *q, &out)) return nullptr;
+  if (!output_arg(call, oo, *q, &out) || (oo != Py_None && !output_apart(call, out, *q, *kc, *vc))) return nullptr;
   if (b && h) {
     const cudaStream_t st = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(call.device)).stream();
     const Scratch ws(mp_paged_attention_decode_workspace_bytes(), call.device, st, kAttention, true);
@@ -743,7 +769,7 @@ PyObject* attention_prefill(PyObject*, PyObject* args) {
   if (PyErr_Occurred()) return nullptr;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(call.device));
   at::Tensor out;
-  if (!output_arg(call, oo, *q, &out)) return nullptr;
+  if (!output_arg(call, oo, *q, &out) || (oo != Py_None && !output_apart(call, out, *q, *k, *v))) return nullptr;
   if (t && h && cu->size(0) > 1) {
     const mp_head_rows qr = head_rows(*q), kr = head_rows(*k), vr = head_rows(*v);
     const int rc = mp_attention_prefill(call.type(), &qr, &kr, &vr, static_cast<int>(t), static_cast<int>(h), static_cast<int>(hk),

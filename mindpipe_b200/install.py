@@ -171,7 +171,9 @@ def install_paged_attention(model: nn.Module, cache: PagedKVCache, *, cos_sin: t
     table is ``cos_sin`` (fp32 ``[positions, rotated]``, cosines then sines) or made from the model's ``rotary_emb``
     (``inv_freq`` and ``attention_scaling``) for ``max_positions`` positions (default: the config's
     ``max_position_embeddings``).  Layers whose attention does more than project, rotate and attend -- normalised
-    queries or keys, sliding windows, capped scores -- raise ``ValueError`` before anything is replaced.
+    queries or keys, sliding windows, capped scores -- or look ahead raise ``ValueError`` before anything is replaced.  The
+    rotation pairs value ``i`` of a head with ``i + rotated / 2``; a model that pairs neighbours is put together from
+    :class:`PagedSelfAttention` with ``interleaved=True``.
     """
     layers, prefix = get_blocks(model), _blocks_prefix(model)
     if len(layers) != cache.pool.shape[0]:
@@ -195,6 +197,8 @@ def install_paged_attention(model: nn.Module, cache: PagedKVCache, *, cos_sin: t
         for extra in ("q_norm", "k_norm", "sliding_window", "attn_logit_softcapping", "sinks"):
             if getattr(attn, extra, None) is not None:
                 raise ValueError(f"{name}: {extra} is not part of the paged attention")
+        if getattr(attn, "is_causal", True) is False:
+            raise ValueError(f"{name}: the paged attention is causal")
         made.append((layer, name, PagedSelfAttention(attn, cache, i, cos_sin, head_dim=getattr(attn, "head_dim", None),
                                                      scale=getattr(attn, "scaling", None))))
     for layer, _, new in made:

@@ -723,7 +723,8 @@ def rotary_append_paged(q, k, v, cos_sin, positions, slots, k_cache, v_cache, *,
     sines; the first ``rotated`` values of a head turn, in pairs ``(i, i + rotated / 2)`` or, with ``interleaved``,
     ``(2i, 2i + 1)``.  Token ``t`` goes to offset ``slots[t] % page_size`` of page ``slots[t] // page_size`` of
     ``k_cache`` / ``v_cache [pages, Hkv, page_size, D]`` (views with other strides included), or nowhere where
-    ``slots[t] < 0`` (padding); a slot may occur once per call.  ``positions`` and ``slots`` are int32 ``[T]``.
+    ``slots[t] < 0`` (padding); a slot may occur once per call (of two tokens with the same one, parts of either may be
+    stored).  ``positions`` and ``slots`` are int32 ``[T]``.  Inference only, as the attention operators: no gradients.
 
     Returns ``(q_rotated, k_rotated | None)``; the caches are updated in place.  Positions and slots out of range touch no
     memory and raise at the next :func:`check_device_errors`.
@@ -741,7 +742,7 @@ def paged_attention_decode(q, k_cache, v_cache, page_table, seq_lens, *, scale: 
     ``q [B,Hq,D]`` fp16 or bf16, ``k_cache`` / ``v_cache [pages, Hkv, page_size, D]`` of the same type (``Hq`` a multiple of
     ``Hkv``), ``page_table`` int32 ``[B, pages of the longest]``, ``seq_lens`` int32 ``[B]``: tokens in the cache, the new
     one included; 0 gives a zero row.  What lies behind a sequence's end, in its last page and in its row of the table, is
-    never read.  ``scale`` defaults to ``D ** -0.5``.  Nothing depends on lengths known to the host: a captured call
+    never read.  ``scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``.  Nothing depends on lengths known to the host: a captured call
     serves whatever lengths the tensor holds at replay.  Pages and lengths out of range raise at the next
     :func:`check_device_errors`.
     """
@@ -757,7 +758,8 @@ def attention_prefill(q, k, v, cu_seqlens, *, scale: float | None = None, out=No
 
     ``q [T,Hq,D]``, ``k`` and ``v [T,Hkv,D]`` fp16 or bf16, strided views included, ``Hq`` a multiple of ``Hkv``;
     ``cu_seqlens`` int32 ``[B + 1]``, ascending, at most ``T``.  Returns ``out [T,Hq,D]``; rows that belong to no sequence
-    are left as they are in ``out``, and unspecified without one.  ``scale`` defaults to ``D ** -0.5``.
+    are left as they are in ``out``, and unspecified without one.  ``scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``,
+    where that is contiguous.
     """
     device = _on_gpu(q, "q")
     y = _lib.host().attention_prefill(q, k, v, cu_seqlens, scale, out, _index_word(device), _error_word(device).data_ptr())
