@@ -13,6 +13,9 @@ shared library (raising if it is missing) and defines
 * ``mindpipe_b200::w8a8_linear(x, weight, weight_scale, bias?) -> y``
 * ``mindpipe_b200::w8a8_gemm(qx, x_scale, weight, weight_scale, bias?) -> y``
 * ``mindpipe_b200::moe_w8a8_experts(hidden, top_k_index, top_k_weights, w13, w13_scale, w2, w2_scale) -> out``
+* ``mindpipe_b200::rotary_append_paged(q, k, v, cos_sin, positions, slots, k_cache!, v_cache!, interleaved) -> (q, k)``
+* ``mindpipe_b200::paged_attention_decode(q, k_cache, v_cache, page_table, seq_lens, scale?) -> out``
+* ``mindpipe_b200::attention_prefill(q, k, v, cu_seqlens, scale?) -> out``
 * ``mindpipe_b200::grouped_swiglu_loop_out(x, weights, batched_weight, group_list, weight_scales,
   batched_weight_scale, x_scale, min_tokens, layer_idx) -> (codes, scales)`` -- the reference's own op name and
   argument list (vllm.patch:114-208)
@@ -99,6 +102,36 @@ def load_and_register():
         @moe_w8a8_experts.register_fake
         def _(hidden, top_k_index, top_k_weights, w13, w13_scale, w2, w2_scale):
             return torch.empty_like(hidden)
+
+        @torch.library.custom_op(f"{NAMESPACE}::rotary_append_paged", mutates_args=("k_cache", "v_cache"))
+        def rotary_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_sin: torch.Tensor,
+                                positions: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
+                                v_cache: torch.Tensor, interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+            return ops.rotary_append_paged(q, k, v, cos_sin, positions, slots, k_cache, v_cache,
+                                           interleaved=interleaved, want_k=True)
+
+        @rotary_append_paged.register_fake
+        def _(q, k, v, cos_sin, positions, slots, k_cache, v_cache, interleaved=False):
+            return q.new_empty(q.shape), k.new_empty(k.shape)
+
+        @torch.library.custom_op(f"{NAMESPACE}::paged_attention_decode", mutates_args=())
+        def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                   page_table: torch.Tensor, seq_lens: torch.Tensor,
+                                   scale: Optional[float] = None) -> torch.Tensor:
+            return ops.paged_attention_decode(q, k_cache, v_cache, page_table, seq_lens, scale=scale)
+
+        @paged_attention_decode.register_fake
+        def _(q, k_cache, v_cache, page_table, seq_lens, scale=None):
+            return q.new_empty(q.shape)
+
+        @torch.library.custom_op(f"{NAMESPACE}::attention_prefill", mutates_args=())
+        def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                              scale: Optional[float] = None) -> torch.Tensor:
+            return ops.attention_prefill(q, k, v, cu_seqlens, scale=scale)
+
+        @attention_prefill.register_fake
+        def _(q, k, v, cu_seqlens, scale=None):
+            return q.new_empty(q.shape)
 
         @torch.library.custom_op(f"{NAMESPACE}::grouped_swiglu_loop_out", mutates_args=())
         def grouped_swiglu_loop_out(x: torch.Tensor, weights: List[torch.Tensor], batched_weight: torch.Tensor,

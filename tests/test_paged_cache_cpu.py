@@ -167,3 +167,46 @@ def test_the_c_entries_check_before_they_touch_a_device():
                        (dict(dtype=2), UNSUPPORTED), (dict(d=130), UNSUPPORTED), (dict(q=rows(token=12)), ALIGNMENT),
                        (dict(out=OK_ARG + 8), ALIGNMENT), (dict(k=rows(token=0)), UNSUPPORTED)):
         assert prefill(**kw) == status, kw
+
+
+def test_bad_bookkeeping_calls_change_nothing():
+    cache = make()
+    a, b = cache.prompts([5, 9]).sequences
+    free = cache.free_pages
+    for bad in ([a, a], [a, 99]):
+        with pytest.raises(KeyError):
+            cache.free(bad)
+        assert cache.free_pages == free and cache.length(a) == 5
+    with pytest.raises(KeyError):
+        cache.next_token([a, 99])
+    assert cache.length(a) == 5
+    for batch, longest in ((0, 10), (2, 0)):
+        with pytest.raises(ValueError):
+            cache.reserve(batch, longest)
+    cache.free([a, b])
+
+
+def test_installer_refuses_attention_that_looks_ahead_or_gates():
+    table = rotary_table(torch.ones(32), 8)
+    for edit in ("is_causal", "o_proj"):
+        model = TinyLlama()
+        attn = model.model.layers[1].self_attn
+        setattr(attn, edit, False if edit == "is_causal" else nn.Linear(128, 256, bias=False))
+        with pytest.raises(ValueError):
+            install.install_paged_attention(model, make(), cos_sin=table)
+        assert not any(isinstance(layer.self_attn, PagedSelfAttention) for layer in model.model.layers)
+
+
+def test_custom_ops_give_shapes_without_a_device():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from mindpipe_b200.custom_ops import load_and_register
+    ns = load_and_register()
+    with FakeTensorMode():
+        qkv = torch.empty(6, 8 * 64, dtype=torch.bfloat16)
+        q, k, v = (x.view(6, -1, 64) for x in qkv.split([256, 128, 128], 1))
+        cache, i = torch.empty(3, 2, 16, 64, dtype=torch.bfloat16), torch.empty(6, dtype=torch.int32)
+        qr, kr = ns.rotary_append_paged(q, k, v, torch.empty(9, 64), i, i, cache, cache)
+        assert qr.shape == q.shape and kr.shape == k.shape and qr.is_contiguous() and qr.dtype == q.dtype
+        assert ns.attention_prefill(q, k, v, torch.empty(2, dtype=torch.int32)).shape == q.shape
+        out = ns.paged_attention_decode(q, cache, cache, torch.empty(6, 2, dtype=torch.int32), i, 0.5)
+        assert out.shape == q.shape and out.is_contiguous()
