@@ -2,19 +2,25 @@
 //
 //   o_i = sum_{j <= i} exp(s_ij - m_i) v_j / sum_{j <= i} exp(s_ij - m_i),   s_ij = scale q_i . k_j
 //
-// with a running maximum, sum and output over tiles of 128 keys.  A block works on two tiles of 128 query rows that share
+// with a running maximum, sum and output over steps of 128 keys.  A block works on two tiles of 128 query rows that share
 // their keys and values -- two heads of a group at the same tokens, or 256 tokens of a head -- so that the tensor cores have
 // one tile's products to do while the other tile's exponentials are taken:
 //
-//   warp 0   copies (TMA): queries, then keys and values in turn through a ring
-//   warp 2   plans: which tiles, ahead of the others
-//   warp 1   tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory
+//   warp 0        copies (TMA): queries, then keys and values in turn through a ring
+//   warp 2        plans: which tiles, ahead of the others
+//   warps 1 and 3 a tile each, tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory (one thread for
+//                 both tiles kept each waiting for the other's weights: 2048 tokens of 32 heads 44.6 us, 42.5 with two)
 //   warps 4-7 and 8-11, one group to a tile: a thread has one row; it takes S from tensor memory, the row's maximum, the
-//            exponentials, and leaves P, rounded, where S was
+//                 exponentials, and leaves P, rounded, where S was
+//
+// A step goes through in two halves of 64 keys, each with its own place for S and P: while one half is multiplied, the
+// exponentials of the other are taken.  (With whole steps a row's chain -- scores, exponentials, product, next scores -- left
+// the exponential unit idle for 1000 of 3300 clocks: 46.2 us.  The products of 64 columns cost the tensor cores a quarter more
+// time, which is why 8192 tokens, at the power limit anyway, gained nothing.)
 //
 // The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights stay in
-// either type's range, the sum is in fp32), so most tiles leave O alone.  Bounds: for heads of 128 values a tile's two
-// products take the tensor cores 1024 clocks and its 16384 exponentials as many.
+// either type's range, the sum is in fp32), so most halves leave O alone.  Bounds: for heads of 128 values a tile's two
+// products of a step take the tensor cores 1300 clocks (1024 at their best), its 16384 exponentials 1024.
 //
 // What a row may not attend to must not reach it, whatever it holds: scores are replaced where masked, but 0 x NaN is NaN in
 // the product with V.  So before the last tile of a sequence's row the group clears rows of V behind the sequence's end and
@@ -28,7 +34,8 @@ using namespace attn;
 using namespace tc;
 
 constexpr int kTile = 128;                     // query rows of a tile and keys of a step
-// Four warps of copies, products, planning and nothing, and two groups of four.  Registers: the block starts with 168 a
+constexpr int kHalf = kTile / 2;               // keys of half a step
+// Four warps of copies, products and planning, and two groups of four.  Registers: the block starts with 168 a
 // thread, 64512 in all; the first four warps give back what the others take, 128 x 72 + 256 x 216 = 64512.
 constexpr int kWarps = 12, kThreads = 32 * kWarps;
 constexpr int kFewRegisters = 72, kManyRegisters = 216;
@@ -45,6 +52,7 @@ struct Prefill {
   static constexpr int kBoxes = DP / 64;                       // copies of 64 columns
   static constexpr int kTileBytes = kTile * DP * 2;
   static constexpr int kStages = 4;
+  static constexpr int kMultiplied = DP == 64 ? 1 : 2;         // of eight pairs of weights
   static constexpr int kBarBytes = 512;
   static constexpr int kOutBytes = 8 * 32 * 128;               // 32 rows of 64 columns for each of eight warps
   static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + kOutBytes + kBarBytes + 1024;
@@ -150,46 +158,57 @@ __device__ __forceinline__ float exp2_ordered(float x) {
   return y;
 }
 
-// Weights 2^(s scale - ref) of 16 scores, their sum added to `sum` and the weights rounded to eight words.  One of the eight
-// pairs is computed by multiplications while the exponential unit has the others: x = n + f with n the nearest integer, 2^f
+// Weights 2^(s scale - ref) of 16 scores, their sum added to `sum` and the weights rounded to eight words.  E of the eight
+// pairs are computed by multiplications while the exponential unit has the others: x = n + f with n the nearest integer, 2^f
 // by a polynomial of degree 5 (minimax on [-1/2, 1/2], found by exchange; relative error 2^-23.6), n added to the exponent.
 // x is at most about 2^7; below -127 it counts as -127, which gives 0.  (A NaN does not come through there: see the maximum.)
 // The unit takes 16 values a clock and SM, 1024 clocks for a tile.  In this order, by hand, the instructions of a warp that
-// is alone on its scheduler keep it busy; as the compiler orders a plain loop they took 1650.  2048 tokens of 32 heads with
-// none, one, two, three of eight by multiplications: 49.2, 48.5, 49.3, 52.9 us.
-// between(m), m = 0..6: what else can be done meanwhile.
-template <typename T, typename F>
+// is alone on its scheduler keep it busy; as the compiler orders a plain loop they took 1650.  With none, one, two of eight by
+// multiplications: 2048 tokens of 32 heads 43.0, 42.5, 41.9 us, 8192 tokens of 64 heads 1085, 1070, 1050; prompts with heads
+// of 64 values, whose products are short, 576, 550, 580.
+// between(m), m < 8 - E: what else can be done meanwhile.
+template <typename T, int E, typename F>
 __device__ __forceinline__ void exp2_batch(const uint32_t* s, F2 scale, F2 minus_ref, F2& sum, uint32_t* packed, F between) {
   constexpr float kMagic = 12582912.0f;        // 1.5 * 2^23: added, the sum's low bits are the nearest integer
   constexpr float kC[6] = {1.3276472454890609e-3f, 9.675540961325169e-3f, 5.550713092088699e-2f,
                            0.24022120237350464f, 0.6931469440460205f, 1.0000001192092896f};
-  F2 x[8], t, f, r;
+  constexpr int U = 8 - E;                     // pairs that the unit takes
+  static_assert(E == 1 || E == 2, "");
+  F2 x[8], t[8], f[8], r[8];
   float v[16];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = fma2(f2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale, minus_ref);
-  {
+#pragma unroll
+  for (int e = U; e < 8; ++e) {
     float a, b;
-    split(x[7], a, b);
-    x[7] = f2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
-    t = add2(x[7], f2(kMagic, kMagic));
+    split(x[e], a, b);
+    x[e] = f2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
+    t[e] = add2(x[e], f2(kMagic, kMagic));
   }
 #pragma unroll
-  for (int m = 0; m < 7; ++m) {
+  for (int m = 0; m < U; ++m) {
     float a, b;
     split(x[m], a, b);
     v[2 * m] = exp2_ordered(a);
     v[2 * m + 1] = exp2_ordered(b);
-    if (m == 0) f = fma2(t, f2(-1.0f, -1.0f), f2(kMagic, kMagic));
-    if (m == 1) f = add2(x[7], f);
-    if (m == 2) r = fma2(f2(kC[0], kC[0]), f, f2(kC[1], kC[1]));
-    if (m > 2) r = fma2(r, f, f2(kC[m - 1], kC[m - 1]));
+#pragma unroll
+    for (int e = U; e < 8; ++e) {
+      const int step = m + 7 - U;              // (of seven; the first two together if there are six turns)
+      if (m == 0) f[e] = fma2(t[e], f2(-1.0f, -1.0f), f2(kMagic, kMagic));
+      if (step == 1) f[e] = add2(x[e], f[e]);
+      if (step == 2) r[e] = fma2(f2(kC[0], kC[0]), f[e], f2(kC[1], kC[1]));
+      if (step > 2 && step <= 6) r[e] = fma2(r[e], f[e], f2(kC[step - 1], kC[step - 1]));
+    }
     between(m);
   }
-  float a, b, t0, t1;
-  split(r, a, b);
-  split(t, t0, t1);
-  v[14] = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
-  v[15] = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
+#pragma unroll
+  for (int e = U; e < 8; ++e) {
+    float a, b, t0, t1;
+    split(r[e], a, b);
+    split(t[e], t0, t1);
+    v[2 * e] = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
+    v[2 * e + 1] = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     sum = add2(sum, f2(v[2 * e], v[2 * e + 1]));
@@ -219,7 +238,7 @@ struct Work {
 
 // The items of a block, in turn, found by a warp.  With up to 256 sequences the tiles of rows are taken by how many keys they
 // have, longest first, and dealt to the blocks back and forth, so that all blocks have about as much to do (one prompt of
-// 2048 tokens and 32 heads: 74 us dealt in one direction, in which case a third of the SMs' time was idle).  With more, in
+// 2048 tokens and 32 heads dealt in one direction: a third of the SMs' time idle).  With more, in
 // the order of the batch.
 struct Planner {
   const PrefillParams& p;
@@ -318,9 +337,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (2 + C::kStages) * C::kTileBytes + C::kOutBytes);
   const uint32_t q_tile = smem_u32(smem), ring = q_tile + 2 * C::kTileBytes;
   const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * C::kStages, q_full = kv_empty + 8 * C::kStages,
-                 q_empty = q_full + 16, s_full = q_empty + 16, p_ready = s_full + 16 /* [tile][half of the keys] */,
-                 o_done = p_ready + 32, scanned = o_done + 16, work_full = scanned + 16, work_empty = work_full + 8 * kAhead;
-  constexpr int kBars = 2 * C::kStages + 14 + 2 * kAhead;
+                 q_empty = q_full + 16, s_full = q_empty + 16 /* [tile][half of the keys] */, p_ready = s_full + 32 /* the same */,
+                 o_done = p_ready + 32 /* the same */, scanned = o_done + 32, work_full = scanned + 16, work_empty = work_full + 8 * kAhead;
+  constexpr int kBars = 2 * C::kStages + 18 + 2 * kAhead;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // [tile][item's parity]: the last product of the tile's item is not the MMA's
@@ -332,21 +351,22 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(kv_full + 8 * s, 1);
-      mbar_init(kv_empty + 8 * s, 1);
+      mbar_init(kv_empty + 8 * s, 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + 8 * i, 1);
       mbar_init(q_empty + 8 * i, 1);
-      mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_ready + 16 * i, 4);
-      mbar_init(p_ready + 16 * i + 8, 4);
-      mbar_init(o_done + 8 * i, 1);
+      for (int half = 0; half < 2; ++half) {
+        mbar_init(s_full + 16 * i + 8 * half, 1);
+        mbar_init(p_ready + 16 * i + 8 * half, 4);
+        mbar_init(o_done + 16 * i + 8 * half, 1);
+      }
       mbar_init(scanned + 8 * i, 4);
       odd_values[2 * i] = odd_values[2 * i + 1] = 0;
     }
     for (int a = 0; a < kAhead; ++a) {
       mbar_init(work_full + 8 * a, 1);
-      mbar_init(work_empty + 8 * a, 10);       // the copying and the multiplying thread, eight warps
+      mbar_init(work_empty + 8 * a, 11);       // the copying and the two multiplying threads, eight warps
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -423,9 +443,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
       }
     }
-    if (warp == 1 && elect_one()) {
+    if ((warp == 1 || warp == 3) && elect_one()) {
+      const int i = warp >> 1;                 // its tile
       constexpr uint32_t kFormats = kIdescDFormatF32 | (__is_same(T, __half) ? 0u : (1u << 7) | (1u << 10));
-      const uint32_t idesc_qk = umma_idesc(kFormats, kTile, kTile) | p.negate;
+      const uint32_t idesc_qk = umma_idesc(kFormats, kTile, kHalf) | p.negate;
       constexpr uint32_t kIdescPV = umma_idesc(kFormats, kTile, DP) | (1u << 16);      // B's rows in memory are K
       const uint64_t k_desc = umma_desc_k_sw128(ring), v_desc = umma_desc_rows_sw128(ring);
       const uint32_t k_lo = static_cast<uint32_t>(k_desc), k_hi = static_cast<uint32_t>(k_desc >> 32);
@@ -437,102 +458,99 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         uint32_t at = 0, phase = 0;
         __device__ __forceinline__ void step(int n) {
           at += n;
-          if (at >= C::kStages) { at -= C::kStages; phase ^= 1; }
+          phase ^= (at / C::kStages) & 1;
+          at %= C::kStages;
         }
       };
-      uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, parity[2] = {0, 0};
+      uint32_t q_phase = 0, p_phase = 0, parity = 0;
       auto full = [&](const Slot& s) { return wait(kv_full + 8 * s.at, s.phase); };
-      auto scores = [&](int i, const Slot& s) {               // S_i = Q_i K^T
-        const uint32_t a = q_lo + i * kTileStep, b = k_lo + s.at * kTileStep;
+      auto scores = [&](const Slot& s, int half) {     // S_i = Q_i K^T, half of the step's keys
+        const uint32_t a = q_lo + i * kTileStep, b = k_lo + s.at * kTileStep + half * ((kHalf * 128) >> 4);
+        const uint32_t d = tmem + i * kTile + half * kHalf;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t at = (k >> 2) * ((kTile * 128) >> 4) + 2 * (k & 3);
-          if (k == 0) umma_ss<false>(tmem + i * kTile, a + at, k_hi, b + at, k_hi, idesc_qk);
-          else umma_ss<true>(tmem + i * kTile, a + at, k_hi, b + at, k_hi, idesc_qk);
+          if (k == 0) umma_ss<false>(d, a + at, k_hi, b + at, k_hi, idesc_qk);
+          else umma_ss<true>(d, a + at, k_hi, b + at, k_hi, idesc_qk);
         }
-        umma_commit(s_full + 8 * i);
+        umma_commit(s_full + 16 * i + 8 * half);
       };
-      auto release = [&](const Slot& s) { umma_commit(kv_empty + 8 * s.at); };
-      int steps[2], then[2];
-      auto take_steps = [&](int (&n)[2]) {     // of the next item
+      // what this tile has used, or has no use for
+      auto release = [&](const Slot& s, bool used) {
+        if (used) umma_commit(kv_empty + 8 * s.at);
+        else if (full(s)) mbar_arrive(kv_empty + 8 * s.at);
+      };
+      int steps, then, most, then_most;
+      auto take_steps = [&]() {                // of the next item
         const int a = taken % kAhead;
         if (!wait(work_full + 8 * a, (taken / kAhead) & 1)) return false;
-        n[0] = works[a].steps[0];
-        n[1] = works[a].steps[1];
+        then = works[a].steps[i];
+        then_most = max(works[a].steps[0], works[a].steps[1]);
+        const bool there = works[a].steps[0] != 0;
         mbar_arrive(work_empty + 8 * a);
         ++taken;
-        return n[0] != 0;
+        return there;
       };
-      // The first scores of an item follow the last product of the one before, tile by tile: the ring's order is that of the
-      // keys' and values' first use by either tile, and it has room for the two or three copies that a tile may be ahead.
-      auto first_scores = [&](int i, int n, const Slot& s) {
-        if (!wait(q_full + 8 * i, q_phase[i]) || !full(s)) return false;
-        q_phase[i] ^= 1;
-        scores(i, s);
-        if (n == 1) umma_commit(q_empty + 8 * i);
+      // The first scores of an item follow the last product of the one before: the ring has room for the two copies that tile 0
+      // may be ahead of tile 1.
+      auto first_scores = [&](const Slot& s, int half) {
+        if (half == 0) {
+          if (!wait(q_full + 8 * i, q_phase)) return false;
+          q_phase ^= 1;
+        }
+        if (!full(s)) return false;
+        scores(s, half);
+        if (half && then == 1) umma_commit(q_empty + 8 * i);
         return true;
       };
-      Slot first;                              // the item's first keys
-      bool more = take_steps(steps), ok = true;
-      if (more) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) ok = ok && (!steps[i] || first_scores(i, steps[i], first));
-        release(first);
-      }
+      Slot k;
+      bool more = take_steps(), ok = true;
+      if (more && then) ok = first_scores(k, 0) && first_scores(k, 1);
       while (ok && more) {
-        more = take_steps(then);
-        const int most = max(steps[0], steps[1]);
-        Slot v = first, k = first, last_k;     // this step's values and the next one's keys, or the next item's
+        steps = then;
+        most = then_most;
+        Slot v = k, next = k;                  // this step's values, the next item's first keys
         v.step(1);
-        k.step(2);
+        next.step(2 * most);
+        release(k, steps != 0);
+        k.step(2);                             // the next step's keys
+        more = take_steps();
         for (int j = 0; ok && j < most; ++j) {
-          if (!full(v)) { ok = false; break; }
+          const bool last = j + 1 >= steps;
+          if (j < steps) {
+            ok = full(v);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (j >= steps[i]) continue;
-            const bool last = j + 1 == steps[i];
-            bool multiply = true;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {            // the weights come in halves of the keys
-              if (!wait(p_ready + 16 * i + 8 * half, p_phase[i])) { ok = false; break; }
+            for (int half = 0; half < 2; ++half) {
+              if (!ok || !wait(p_ready + 16 * i + 8 * half, p_phase)) { ok = false; continue; }
               tcgen05_fence_after();
-              if (half == 0 && last) multiply = odd_values[2 * i + parity[i]] == 0;
-              if (multiply) {
+              if (!last || odd_values[2 * i + parity] == 0) {
                 const uint32_t b = v_lo + v.at * kTileStep;
 #pragma unroll
                 for (int k = 4 * half; k < 4 * half + 4; ++k)
-                  umma_ts(tmem + 2 * kTile + i * DP, tmem + i * kTile + k * 8, b + k * ((16 * 128) >> 4), v_hi, kIdescPV, k != 0 ? 1u : j != 0);
+                  umma_ts(tmem + 2 * kTile + i * DP, tmem + i * kTile + half * kHalf + (k & 3) * 8, b + k * ((16 * 128) >> 4), v_hi, kIdescPV, k != 0 ? 1u : j != 0);
+              }
+              umma_commit(o_done + 16 * i + 8 * half);
+              if (!last) {
+                ok = full(k);
+                if (ok) scores(k, half);
+                if (half && j + 2 == steps) umma_commit(q_empty + 8 * i);
+              } else if (more && then) {
+                ok = first_scores(next, half);
               }
             }
+            p_phase ^= 1;
+            if (last) parity ^= 1;
             if (!ok) break;
-            p_phase[i] ^= 1;
-            umma_commit(o_done + 8 * i);
-            if (!last) {
-              if (!full(k)) { ok = false; break; }
-              scores(i, k);
-              if (j + 2 == steps[i]) umma_commit(q_empty + 8 * i);
-            } else {
-              parity[i] ^= 1;
-              if (more && then[i]) {
-                Slot next = k;                 // the next item's first keys: two copies on if tile 1 has one step more
-                if (j + 1 < most) next.step(2);
-                if (!first_scores(i, then[i], next)) { ok = false; break; }
-              }
-            }
           }
-          if (!ok) break;
-          release(v);
-          if (j + 1 < most) release(k);
-          last_k = k;
+          release(v, j < steps);
+          if (j + 1 < most) {
+            release(k, !last);
+            k.step(2);
+          }
           v.step(2);
-          k.step(2);
         }
-        if (!ok || !more) break;
-        first = last_k;
-        if (!steps[1] && then[1] && !first_scores(1, then[1], first)) break;
-        release(first);
-        steps[0] = then[0];
-        steps[1] = then[1];
+        k = next;
+        if (ok && more && !steps && then) ok = first_scores(k, 0) && first_scores(k, 1);
       }
     }
     if (warp == 2) {
@@ -556,7 +574,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const int i = warp >= 8, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + i * kTile, o_tmem = tmem + lanes + 2 * kTile + i * DP;
-    uint32_t s_phase = 0, o_phase = 0, scan_phase = 0;         // o_phase: of the next product to complete
+    uint32_t turn = 0, scan_phase = 0;         // parity of the steps so far, which is that of their scores and products
     int load = 0;
     bool ok = true;
     const F2 scale2 = f2(p.scale_log2, p.scale_log2);
@@ -576,23 +594,28 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       load += 2 * item_steps;
       if (!steps) continue;
       float m = kNegInf, sum = 0.0f;
-      for (int j = 0; j < steps; ++j) {
-        if (!wait_all(s_full + 8 * i, s_phase)) { ok = false; break; }
-        s_phase ^= 1;
+      uint32_t tile_v = 0;                     // of the last step
+#pragma unroll 1
+      for (int h = 0; h < 2 * steps; ++h) {    // halves of a step's keys
+        const int half = h & 1;
+        const uint32_t s_half = s_tmem + half * kHalf;
+        // the tile's product before this half's: of the step before, or of its first half
+        auto wait_before = [&]() { return wait_all(o_done + 16 * i + 8 * (half ^ 1), turn ^ (half ^ 1)); };
+        if (!wait_all(s_full + 16 * i + 8 * half, turn)) { ok = false; break; }
         tcgen05_fence_after();
-        const bool last = j + 1 == steps;
-        uint32_t s[4][32];
+        const bool last = h + 2 >= 2 * steps;
+        uint32_t s[2][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_tmem + 32 * c, s[c]);
+        for (int c = 0; c < 2; ++c) tmem_ld_32x32(s_half + 32 * c, s[c]);
         tmem_ld_wait();
         auto value = [&](int c) -> uint32_t& { return s[c >> 5][c & 31]; };
         if (last) {
 #pragma unroll
-          for (int c = 0; c < kTile; ++c) value(c) = c <= row ? value(c) : __float_as_uint(kNegInf);
+          for (int c = 0; c < kHalf; ++c) value(c) = half * kHalf + c <= row ? value(c) : __float_as_uint(kNegInf);
         }
-        // The weights are taken with the maximum of the steps before (the first step's own at first): it is still good if no
-        // score exceeds it by 8.  The scores' maximum is found beside the first half's exponentials; where it exceeds, the
-        // half is taken once more.  A NaN anywhere makes the maximum NaN, and with it the whole row; so does plus infinity.
+        // The weights are taken with the maximum of the halves before (the first one's own at first): it is still good if no
+        // score exceeds it by 8.  The scores' maximum is found beside the exponentials; where it exceeds, they are taken once
+        // more.  A NaN anywhere makes the maximum NaN, and with it the whole row; so does plus infinity.
         float top[4];
         auto look = [&](int c) {
 #pragma unroll
@@ -601,26 +624,25 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         };
         auto maximum = [&]() { return max3(m, max3(top[0], top[1], top[2]) * p.scale_log2, top[3] * p.scale_log2); };
         auto usable = [&](float now) { return now == -kNegInf ? __uint_as_float(0x7fffffffu) : now; };
-        if (j == 0) {
+        if (h == 0) {
 #pragma unroll
-          for (int c = 0; c < kTile; c += 8) look(c);
+          for (int c = 0; c < kHalf; c += 8) look(c);
           m = usable(maximum());
         }
-        F2 part, minus_ref;
+        F2 part;
         uint32_t packed[32];
-        for (bool again = j == 0;; again = true) {
+        for (bool again = h == 0;; again = true) {
           const float ref = m == kNegInf ? 0.0f : m;
-          minus_ref = f2(kLift<T> - ref, kLift<T> - ref);
+          const F2 minus_ref = f2(kLift<T> - ref, kLift<T> - ref);
           part = 0;
 #pragma unroll
           for (int b = 0; b < 4; ++b)
-            exp2_batch<T>(&value(16 * b), scale2, minus_ref, part, packed + 8 * b, [&](int step) {
-              if (step < 4) look(32 * b + 8 * step);
+            exp2_batch<T, C::kMultiplied>(&value(16 * b), scale2, minus_ref, part, packed + 8 * b, [&](int step) {
+              if (step < 2) look(16 * b + 8 * step);
             });
           const float now = maximum();
           if (again || !__any_sync(0xffffffffu, !(now <= m + kGrowth))) break;
-          // (number j + 1 is the product of this tile that is the next to complete)
-          if (!wait_all(o_done + 8 * i, o_phase ^ 1)) { ok = false; break; }      // product j
+          if (!wait_before()) { ok = false; break; }
           tcgen05_fence_after();
           const float grown = usable(now), keep = grown == kNegInf ? 1.0f : exp2_fast(m - grown);
           sum *= keep;
@@ -636,25 +658,15 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           }
         }
         if (!ok) break;
-        o_phase ^= 1;
-        tmem_st_32x32(s_tmem, packed);
-        if (!last) {                           // the product with the first half of the keys may begin
-          tmem_st_wait();
-          tcgen05_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(p_ready + 16 * i);
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) exp2_batch<T>(&value(64 + 16 * b), scale2, minus_ref, part, packed + 8 * b, [](int) {});
-        tmem_st_32x32(s_tmem + 32, packed);
+        tmem_st_32x32(s_half, packed);
         float part_sum[2];
         split(part, part_sum[0], part_sum[1]);
         sum += part_sum[0] + part_sum[1];
-        if (last) {
+        if (last && half == 0) {
           // ---- V's rows behind the sequence's end, and values that are not finite
-          const int n = first_load + 2 * j + 1, valid = len - j * kTile;
+          const int n = first_load + h + 1, valid = len - h * kHalf;
           if (!wait_all(kv_full + 8 * (n % C::kStages), (n / C::kStages) & 1)) { ok = false; break; }
-          const uint32_t tile_v = ring + (n % C::kStages) * C::kTileBytes;
+          tile_v = ring + (n % C::kStages) * C::kTileBytes;
           uint32_t zeros = 0;
 #pragma unroll 2
           for (int c = 0; c < 8 * C::kBoxes; ++c) {
@@ -670,59 +682,58 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           mbar_arrive_warp(scanned + 8 * i, lane);
           if (!wait_all(scanned + 8 * i, scan_phase)) { ok = false; break; }
           scan_phase ^= 1;
-          if (odd_values[2 * i + (scan_phase ^ 1)]) {
-            // this row's product with the keys it attends to, 32 columns at a time
-            tmem_st_wait();
-            if (j > 0) {
-              if (!wait_all(o_done + 8 * i, o_phase)) { ok = false; break; }      // product j, of the tile before
-              tcgen05_fence_after();
+        }
+        if (last && odd_values[2 * i + (scan_phase ^ 1)]) {
+          // this row's product with the keys it attends to, 32 columns at a time
+          tmem_st_wait();
+          if (h > 0) {
+            if (!wait_before()) { ok = false; break; }
+            tcgen05_fence_after();
+          }
+#pragma unroll 1
+          for (int d0 = 0; d0 < DP; d0 += 32) {
+            uint32_t o[32];
+            if (h > 0) {
+              tmem_ld_32x32(o_tmem + d0, o);
+              tmem_ld_wait();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = 0u;
             }
 #pragma unroll 1
-            for (int d0 = 0; d0 < DP; d0 += 32) {
-              uint32_t o[32];
-              if (j > 0) {
-                tmem_ld_32x32(o_tmem + d0, o);
-                tmem_ld_wait();
-              } else {
+            for (int c = 0; c < kHalf; c += 2) {
+              const float2 pair = unpack2<T>(tmem_ld_column(s_half + c / 2));
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0u;
-              }
-#pragma unroll 1
-              for (int c = 0; c < kTile; c += 2) {
-                const float2 pair = unpack2<T>(tmem_ld_column(s_tmem + c / 2));
+              for (int k = 0; k < 2; ++k) {
+                const int key = half * kHalf + c + k;
+                if (key > row) continue;
+                const float weight = k ? pair.y : pair.x;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  if (c + k > row) continue;
-                  const float weight = k ? pair.y : pair.x;
+                for (int e = 0; e < 4; ++e) {
+                  const uint4 v = lds16(tile_v + (d0 >> 6) * kTile * 128 + key * 128 + ((((d0 & 63) / 8 + e) ^ (key & 7)) << 4));
+                  const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    const uint4 v = lds16(tile_v + (d0 >> 6) * kTile * 128 + (c + k) * 128 + ((((d0 & 63) / 8 + e) ^ ((c + k) & 7)) << 4));
-                    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                      const float2 y = unpack2<T>(words[x]);
-                      uint32_t &o0 = o[e * 8 + 2 * x], &o1 = o[e * 8 + 2 * x + 1];
-                      o0 = __float_as_uint(fmaf(weight, y.x, __uint_as_float(o0)));
-                      o1 = __float_as_uint(fmaf(weight, y.y, __uint_as_float(o1)));
-                    }
+                  for (int x = 0; x < 4; ++x) {
+                    const float2 y = unpack2<T>(words[x]);
+                    uint32_t &o0 = o[e * 8 + 2 * x], &o1 = o[e * 8 + 2 * x + 1];
+                    o0 = __float_as_uint(fmaf(weight, y.x, __uint_as_float(o0)));
+                    o1 = __float_as_uint(fmaf(weight, y.y, __uint_as_float(o1)));
                   }
                 }
               }
-              tmem_st_32x32(o_tmem + d0, o);
             }
+            tmem_st_32x32(o_tmem + d0, o);
           }
         }
         tmem_st_wait();
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (last) mbar_arrive(p_ready + 16 * i);
-          mbar_arrive(p_ready + 16 * i + 8);
-        }
+        if (lane == 0) mbar_arrive(p_ready + 16 * i + 8 * half);
+        turn ^= half;
       }
       if (!ok) break;
       // ---- the row's result
-      if (!wait_all(o_done + 8 * i, o_phase ^ 1)) { ok = false; break; }
+      if (!wait_all(o_done + 16 * i + 8, turn ^ 1)) { ok = false; break; }
       tcgen05_fence_after();
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       // 64 columns at a time through shared memory, so that a warp's stores are whole lines (a row to a thread took 3000 clocks
