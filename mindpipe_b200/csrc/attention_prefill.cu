@@ -9,22 +9,25 @@
 //   warp 0        copies (TMA): queries, then keys and values in turn through a ring
 //   warp 2        plans: which tiles, ahead of the others
 //   warps 1 and 3 a tile each, tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory (one thread for
-//                 both tiles kept each waiting for the other's weights: 2048 tokens of 32 heads 44.6 us, 42.5 with two)
+//                 both kept each waiting for the other's weights: 2048 tokens of 32 heads 44.6 us, 42.5 with two)
 //   warps 4-7 and 8-11, one group to a tile: a thread has one row; it takes S from tensor memory, the row's maximum, the
 //                 exponentials, and leaves P, rounded, where S was
 //
-// A step goes through in two halves of 64 keys, each with its own place for S and P: while one half is multiplied, the
-// exponentials of the other are taken.  (With whole steps a row's chain -- scores, exponentials, product, next scores -- left
-// the exponential unit idle for 1000 of 3300 clocks: 46.2 us.  The products of 64 columns cost the tensor cores a quarter more
-// time, which is why 8192 tokens, at the power limit anyway, gained nothing.)
+// Scores, exponentials, product and next scores are a chain for each row; so that the exponential unit is not left waiting for
+// the tensor cores, the next scores have to be there when a group is done.  Tensor memory has 512 columns.  With heads of 128
+// values S and O take all of it, and a step goes through in two halves of 64 keys, each with its own place for S and P: while
+// one half is multiplied, the exponentials of the other are taken.  (2048 tokens of 32 heads in whole steps 46.2 us, in halves
+// 42.5.  The products of 64 columns cost the tensor cores a quarter more time, which is why 8192 tokens, at the power limit
+// anyway, gained nothing: 1030, 1050.)  With heads of 64 values there is room for P beside S, and the next scores are sent for
+// as soon as these are read (whole steps with P in S's place 540 us, halves 549, P apart 527).
 //
 // The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights stay in
-// either type's range, the sum is in fp32), so most halves leave O alone.  Bounds: for heads of 128 values a tile's two
+// either type's range, the sum is in fp32), so most steps leave O alone.  Bounds: for heads of 128 values a tile's two
 // products of a step take the tensor cores 1300 clocks (1024 at their best), its 16384 exponentials 1024.
 //
 // What a row may not attend to must not reach it, whatever it holds: scores are replaced where masked, but 0 x NaN is NaN in
-// the product with V.  So before the last tile of a sequence's row the group clears rows of V behind the sequence's end and
-// looks for values that are not finite; where there are any, the threads add that tile's product up themselves.
+// the product with V.  So before the last step of a tile's rows the group clears rows of V behind the sequence's end and
+// looks for values that are not finite; where there are any, the threads add that step's product up themselves.
 #include "attention.cuh"
 
 namespace mp {
@@ -34,7 +37,6 @@ using namespace attn;
 using namespace tc;
 
 constexpr int kTile = 128;                     // query rows of a tile and keys of a step
-constexpr int kHalf = kTile / 2;               // keys of half a step
 // Four warps of copies, products and planning, and two groups of four.  Registers: the block starts with 168 a
 // thread, 64512 in all; the first four warps give back what the others take, 128 x 72 + 256 x 216 = 64512.
 constexpr int kWarps = 12, kThreads = 32 * kWarps;
@@ -52,6 +54,11 @@ struct Prefill {
   static constexpr int kBoxes = DP / 64;                       // copies of 64 columns
   static constexpr int kTileBytes = kTile * DP * 2;
   static constexpr int kStages = 4;
+  // P beside S, and a step in one part; or a step in two, whose weights take their scores' place
+  static constexpr bool kApart = DP == 64;
+  static constexpr int kParts = kApart ? 1 : 2, kPart = kTile / kParts;
+  // tensor memory: S of either tile, O of either tile, and P
+  static constexpr int kWeights = kApart ? 2 * (kTile + DP) : 0, kWeightStep = kApart ? kTile / 2 : kTile;
   static constexpr int kMultiplied = DP == 64 ? 1 : 2;         // of eight pairs of weights
   static constexpr int kBarBytes = 512;
   static constexpr int kOutBytes = 8 * 32 * 128;               // 32 rows of 64 columns for each of eight warps
@@ -165,7 +172,7 @@ __device__ __forceinline__ float exp2_ordered(float x) {
 // The unit takes 16 values a clock and SM, 1024 clocks for a tile.  In this order, by hand, the instructions of a warp that
 // is alone on its scheduler keep it busy; as the compiler orders a plain loop they took 1650.  With none, one, two of eight by
 // multiplications: 2048 tokens of 32 heads 43.0, 42.5, 41.9 us, 8192 tokens of 64 heads 1085, 1070, 1050; prompts with heads
-// of 64 values, whose products are short, 576, 550, 580.
+// of 64 values, whose products are short, with one or two 527, 549.
 // between(m), m < 8 - E: what else can be done meanwhile.
 template <typename T, int E, typename F>
 __device__ __forceinline__ void exp2_batch(const uint32_t* s, F2 scale, F2 minus_ref, F2& sum, uint32_t* packed, F between) {
@@ -337,9 +344,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (2 + C::kStages) * C::kTileBytes + C::kOutBytes);
   const uint32_t q_tile = smem_u32(smem), ring = q_tile + 2 * C::kTileBytes;
   const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * C::kStages, q_full = kv_empty + 8 * C::kStages,
-                 q_empty = q_full + 16, s_full = q_empty + 16 /* [tile][half of the keys] */, p_ready = s_full + 32 /* the same */,
-                 o_done = p_ready + 32 /* the same */, scanned = o_done + 32, work_full = scanned + 16, work_empty = work_full + 8 * kAhead;
-  constexpr int kBars = 2 * C::kStages + 18 + 2 * kAhead;
+                 q_empty = q_full + 16, s_full = q_empty + 16 /* [tile][part of the step] */, p_ready = s_full + 32 /* the same */,
+                 o_done = p_ready + 32 /* the same */, scanned = o_done + 32, s_read = scanned + 16, work_full = s_read + 16, work_empty = work_full + 8 * kAhead;
+  constexpr int kBars = 2 * C::kStages + 20 + 2 * kAhead;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // [tile][item's parity]: the last product of the tile's item is not the MMA's
@@ -356,11 +363,12 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + 8 * i, 1);
       mbar_init(q_empty + 8 * i, 1);
-      for (int half = 0; half < 2; ++half) {
-        mbar_init(s_full + 16 * i + 8 * half, 1);
-        mbar_init(p_ready + 16 * i + 8 * half, 4);
-        mbar_init(o_done + 16 * i + 8 * half, 1);
+      for (int part = 0; part < 2; ++part) {
+        mbar_init(s_full + 16 * i + 8 * part, 1);
+        mbar_init(p_ready + 16 * i + 8 * part, 4);
+        mbar_init(o_done + 16 * i + 8 * part, 1);
       }
+      mbar_init(s_read + 8 * i, 4);
       mbar_init(scanned + 8 * i, 4);
       odd_values[2 * i] = odd_values[2 * i + 1] = 0;
     }
@@ -446,7 +454,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     if ((warp == 1 || warp == 3) && elect_one()) {
       const int i = warp >> 1;                 // its tile
       constexpr uint32_t kFormats = kIdescDFormatF32 | (__is_same(T, __half) ? 0u : (1u << 7) | (1u << 10));
-      const uint32_t idesc_qk = umma_idesc(kFormats, kTile, kHalf) | p.negate;
+      const uint32_t idesc_qk = umma_idesc(kFormats, kTile, C::kPart) | p.negate;
       constexpr uint32_t kIdescPV = umma_idesc(kFormats, kTile, DP) | (1u << 16);      // B's rows in memory are K
       const uint64_t k_desc = umma_desc_k_sw128(ring), v_desc = umma_desc_rows_sw128(ring);
       const uint32_t k_lo = static_cast<uint32_t>(k_desc), k_hi = static_cast<uint32_t>(k_desc >> 32);
@@ -464,16 +472,16 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       };
       uint32_t q_phase = 0, p_phase = 0, parity = 0;
       auto full = [&](const Slot& s) { return wait(kv_full + 8 * s.at, s.phase); };
-      auto scores = [&](const Slot& s, int half) {     // S_i = Q_i K^T, half of the step's keys
-        const uint32_t a = q_lo + i * kTileStep, b = k_lo + s.at * kTileStep + half * ((kHalf * 128) >> 4);
-        const uint32_t d = tmem + i * kTile + half * kHalf;
+      auto scores = [&](const Slot& s, int part) {            // S_i = Q_i K^T of a part of the step's keys
+        const uint32_t a = q_lo + i * kTileStep, b = k_lo + s.at * kTileStep + part * ((C::kPart * 128) >> 4);
+        const uint32_t d = tmem + i * kTile + part * C::kPart;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t at = (k >> 2) * ((kTile * 128) >> 4) + 2 * (k & 3);
           if (k == 0) umma_ss<false>(d, a + at, k_hi, b + at, k_hi, idesc_qk);
           else umma_ss<true>(d, a + at, k_hi, b + at, k_hi, idesc_qk);
         }
-        umma_commit(s_full + 16 * i + 8 * half);
+        umma_commit(s_full + 16 * i + 8 * part);
       };
       // what this tile has used, or has no use for
       auto release = [&](const Slot& s, bool used) {
@@ -493,19 +501,20 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       };
       // The first scores of an item follow the last product of the one before: the ring has room for the two copies that tile 0
       // may be ahead of tile 1.
-      auto first_scores = [&](const Slot& s, int half) {
-        if (half == 0) {
+      auto first_scores = [&](const Slot& s, int part) {
+        if (part == 0) {
           if (!wait(q_full + 8 * i, q_phase)) return false;
           q_phase ^= 1;
         }
         if (!full(s)) return false;
-        scores(s, half);
-        if (half && then == 1) umma_commit(q_empty + 8 * i);
+        scores(s, part);
+        if (part + 1 == C::kParts && then == 1) umma_commit(q_empty + 8 * i);
         return true;
       };
+      auto all_first_scores = [&](const Slot& s) { return first_scores(s, 0) && (C::kParts == 1 || first_scores(s, 1)); };
       Slot k;
       bool more = take_steps(), ok = true;
-      if (more && then) ok = first_scores(k, 0) && first_scores(k, 1);
+      if (more && then) ok = all_first_scores(k);
       while (ok && more) {
         steps = then;
         most = then_most;
@@ -518,24 +527,34 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         for (int j = 0; ok && j < most; ++j) {
           const bool last = j + 1 >= steps;
           if (j < steps) {
-            ok = full(v);
+            auto next_scores = [&](int part) {
+              if (!full(k)) return false;
+              scores(k, part);
+              if (part + 1 == C::kParts && j + 2 == steps) umma_commit(q_empty + 8 * i);
+              return true;
+            };
+            if (C::kApart) {                   // (S of this step has been read)
+              ok = wait(s_read + 8 * i, p_phase);
+              tcgen05_fence_after();
+              if (ok && !last) ok = next_scores(0);
+            }
+            ok = ok && full(v);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              if (!ok || !wait(p_ready + 16 * i + 8 * half, p_phase)) { ok = false; continue; }
+            for (int part = 0; part < C::kParts; ++part) {
+              if (!ok || !wait(p_ready + 16 * i + 8 * part, p_phase)) { ok = false; continue; }
               tcgen05_fence_after();
               if (!last || odd_values[2 * i + parity] == 0) {
-                const uint32_t b = v_lo + v.at * kTileStep;
+                const uint32_t b = v_lo + v.at * kTileStep + part * (C::kPart * 128 >> 4);
 #pragma unroll
-                for (int k = 4 * half; k < 4 * half + 4; ++k)
-                  umma_ts(tmem + 2 * kTile + i * DP, tmem + i * kTile + half * kHalf + (k & 3) * 8, b + k * ((16 * 128) >> 4), v_hi, kIdescPV, k != 0 ? 1u : j != 0);
+                for (int k = 0; k < C::kPart / 16; ++k)
+                  umma_ts(tmem + 2 * kTile + i * DP, tmem + C::kWeights + i * C::kWeightStep + part * C::kPart + k * 8,
+                          b + k * ((16 * 128) >> 4), v_hi, kIdescPV, part + k != 0 ? 1u : j != 0);
               }
-              umma_commit(o_done + 16 * i + 8 * half);
+              umma_commit(o_done + 16 * i + 8 * part);
               if (!last) {
-                ok = full(k);
-                if (ok) scores(k, half);
-                if (half && j + 2 == steps) umma_commit(q_empty + 8 * i);
+                if (!C::kApart) ok = next_scores(part);
               } else if (more && then) {
-                ok = first_scores(next, half);
+                ok = first_scores(next, part);
               }
             }
             p_phase ^= 1;
@@ -550,7 +569,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           v.step(2);
         }
         k = next;
-        if (ok && more && !steps && then) ok = first_scores(k, 0) && first_scores(k, 1);
+        if (ok && more && !steps && then) ok = all_first_scores(k);
       }
     }
     if (warp == 2) {
@@ -574,6 +593,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const int i = warp >= 8, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + i * kTile, o_tmem = tmem + lanes + 2 * kTile + i * DP;
+    const uint32_t p_tmem = tmem + lanes + C::kWeights + i * C::kWeightStep;
     uint32_t turn = 0, scan_phase = 0;         // parity of the steps so far, which is that of their scores and products
     int load = 0;
     bool ok = true;
@@ -596,24 +616,31 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       float m = kNegInf, sum = 0.0f;
       uint32_t tile_v = 0;                     // of the last step
 #pragma unroll 1
-      for (int h = 0; h < 2 * steps; ++h) {    // halves of a step's keys
-        const int half = h & 1;
-        const uint32_t s_half = s_tmem + half * kHalf;
-        // the tile's product before this half's: of the step before, or of its first half
-        auto wait_before = [&]() { return wait_all(o_done + 16 * i + 8 * (half ^ 1), turn ^ (half ^ 1)); };
-        if (!wait_all(s_full + 16 * i + 8 * half, turn)) { ok = false; break; }
+      for (int h = 0; h < C::kParts * steps; ++h) {
+        const int part = C::kParts == 1 ? 0 : h & 1;
+        const uint32_t p_part = p_tmem + part * C::kPart;
+        // the tile's product before this part's: of the step before, or of its first half
+        auto wait_before = [&]() {
+          if (C::kParts == 1) return wait_all(o_done + 16 * i, turn ^ 1);
+          return wait_all(o_done + 16 * i + 8 * (part ^ 1), turn ^ (part ^ 1));
+        };
+        if (!wait_all(s_full + 16 * i + 8 * part, turn)) { ok = false; break; }
         tcgen05_fence_after();
-        const bool last = h + 2 >= 2 * steps;
-        uint32_t s[2][32];
+        const bool last = h + C::kParts >= C::kParts * steps;
+        uint32_t s[C::kPart / 32][32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) tmem_ld_32x32(s_half + 32 * c, s[c]);
+        for (int c = 0; c < C::kPart / 32; ++c) tmem_ld_32x32(s_tmem + part * C::kPart + 32 * c, s[c]);
         tmem_ld_wait();
+        if (C::kApart) {
+          tcgen05_fence_before();
+          mbar_arrive_warp(s_read + 8 * i, lane);
+        }
         auto value = [&](int c) -> uint32_t& { return s[c >> 5][c & 31]; };
         if (last) {
 #pragma unroll
-          for (int c = 0; c < kHalf; ++c) value(c) = half * kHalf + c <= row ? value(c) : __float_as_uint(kNegInf);
+          for (int c = 0; c < C::kPart; ++c) value(c) = part * C::kPart + c <= row ? value(c) : __float_as_uint(kNegInf);
         }
-        // The weights are taken with the maximum of the halves before (the first one's own at first): it is still good if no
+        // The weights are taken with the maximum of the parts before (the first one's own at first): it is still good if no
         // score exceeds it by 8.  The scores' maximum is found beside the exponentials; where it exceeds, they are taken once
         // more.  A NaN anywhere makes the maximum NaN, and with it the whole row; so does plus infinity.
         float top[4];
@@ -626,19 +653,19 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         auto usable = [&](float now) { return now == -kNegInf ? __uint_as_float(0x7fffffffu) : now; };
         if (h == 0) {
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 8) look(c);
+          for (int c = 0; c < C::kPart; c += 8) look(c);
           m = usable(maximum());
         }
-        F2 part;
+        F2 weights, minus_ref;
         uint32_t packed[32];
         for (bool again = h == 0;; again = true) {
           const float ref = m == kNegInf ? 0.0f : m;
-          const F2 minus_ref = f2(kLift<T> - ref, kLift<T> - ref);
-          part = 0;
+          minus_ref = f2(kLift<T> - ref, kLift<T> - ref);
+          weights = 0;
 #pragma unroll
           for (int b = 0; b < 4; ++b)
-            exp2_batch<T, C::kMultiplied>(&value(16 * b), scale2, minus_ref, part, packed + 8 * b, [&](int step) {
-              if (step < 2) look(16 * b + 8 * step);
+            exp2_batch<T, C::kMultiplied>(&value(16 * b), scale2, minus_ref, weights, packed + 8 * b, [&](int step) {
+              if (step < C::kPart / 32) look(C::kPart / 4 * b + 8 * step);
             });
           const float now = maximum();
           if (again || !__any_sync(0xffffffffu, !(now <= m + kGrowth))) break;
@@ -658,13 +685,20 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           }
         }
         if (!ok) break;
-        tmem_st_32x32(s_half, packed);
-        float part_sum[2];
-        split(part, part_sum[0], part_sum[1]);
-        sum += part_sum[0] + part_sum[1];
-        if (last && half == 0) {
+        if (C::kApart && !wait_before()) { ok = false; break; }        // P of the step before has been used
+        tmem_st_32x32(p_part, packed);
+        if (C::kPart == 128) {
+#pragma unroll
+          for (int b = 4; b < C::kPart / 16; ++b)
+            exp2_batch<T, C::kMultiplied>(&value(16 * b), scale2, minus_ref, weights, packed + 8 * (b - 4), [](int) {});
+          tmem_st_32x32(p_part + 32, packed);
+        }
+        float weight[2];
+        split(weights, weight[0], weight[1]);
+        sum += weight[0] + weight[1];
+        if (last && part == 0) {
           // ---- V's rows behind the sequence's end, and values that are not finite
-          const int n = first_load + h + 1, valid = len - h * kHalf;
+          const int n = first_load + 2 * h / C::kParts + 1, valid = len - h * C::kPart;
           if (!wait_all(kv_full + 8 * (n % C::kStages), (n / C::kStages) & 1)) { ok = false; break; }
           tile_v = ring + (n % C::kStages) * C::kTileBytes;
           uint32_t zeros = 0;
@@ -701,11 +735,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
               for (int e = 0; e < 32; ++e) o[e] = 0u;
             }
 #pragma unroll 1
-            for (int c = 0; c < kHalf; c += 2) {
-              const float2 pair = unpack2<T>(tmem_ld_column(s_half + c / 2));
+            for (int c = 0; c < C::kPart; c += 2) {
+              const float2 pair = unpack2<T>(tmem_ld_column(p_part + c / 2));
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                const int key = half * kHalf + c + k;
+                const int key = part * C::kPart + c + k;
                 if (key > row) continue;
                 const float weight = k ? pair.y : pair.x;
 #pragma unroll
@@ -728,12 +762,12 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tmem_st_wait();
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready + 16 * i + 8 * half);
-        turn ^= half;
+        if (lane == 0) mbar_arrive(p_ready + 16 * i + 8 * part);
+        if (part + 1 == C::kParts) turn ^= 1;
       }
       if (!ok) break;
       // ---- the row's result
-      if (!wait_all(o_done + 16 * i + 8, turn ^ 1)) { ok = false; break; }
+      if (!wait_all(o_done + 16 * i + 8 * (C::kParts - 1), turn ^ 1)) { ok = false; break; }
       tcgen05_fence_after();
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       // 64 columns at a time through shared memory, so that a warp's stores are whole lines (a row to a thread took 3000 clocks
