@@ -16,10 +16,10 @@
 // Scores, exponentials, product and next scores are a chain for each row; so that the exponential unit is not left waiting for
 // the tensor cores, the next scores have to be there when a group is done.  Tensor memory has 512 columns.  With heads of 128
 // values S and O take all of it, and a step goes through in two halves of 64 keys, each with its own place for S and P: while
-// one half is multiplied, the exponentials of the other are taken.  (2048 tokens of 32 heads in whole steps 46.2 us, in halves
-// 42.5.  The products of 64 columns cost the tensor cores a quarter more time, which is why 8192 tokens, at the power limit
-// anyway, gained nothing: 1030, 1050.)  With heads of 64 values there is room for P beside S, and the next scores are sent for
-// as soon as these are read (whole steps with P in S's place 540 us, halves 549, P apart 527).
+// one half is multiplied, the exponentials of the other are taken.  (2048 tokens of 32 heads: in whole steps 46.4 us, in
+// halves 41.5.  The products of 64 columns cost the tensor cores a quarter more time, which is why 8192 tokens of 64 heads, at
+// the power limit anyway, gained nothing: 1013, 1031.)  With heads of 64 values there is room for P beside S, and the next
+// scores are sent for as soon as these are read (whole steps with P in S's place 540 us, halves 549, P apart 528).
 //
 // The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights stay in
 // either type's range, the sum is in fp32), so most steps leave O alone.  Bounds: for heads of 128 values a tile's two
