@@ -777,7 +777,7 @@ typedef struct {
  * then their sines.  Pairs are (i, i + rotated / 2), or (2i, 2i + 1) with interleaved != 0; arithmetic in fp32, one
  * rounding.  q_out [T,Hq,D] and, unless null, k_out [T,Hkv,D] get the rotated queries and keys.  2 <= rotated <= D, even.
  * A token with a negative slot may have any position; one out of range then counts as 0.  Slots that occur twice
- * in a call are left with values of either token.  q_out and k_out may not overlap the inputs.
+ * in a call are left with values of either token.  q_out and k_out may not overlap the inputs, nor these the cache.
  */
 int mp_rotary_append_paged(int dtype, const mp_head_rows* q, const mp_head_rows* k, const mp_head_rows* v,
                            const void* cos_sin_f32, int max_positions, int rotated, int interleaved,
@@ -789,7 +789,7 @@ int mp_rotary_append_paged(int dtype, const mp_head_rows* q, const mp_head_rows*
  * (int32 [B, table_pages], entries behind the last token's page are not read); seq_lens[b] == 0 gives zeros.  Query head i
  * attends to the keys of head i / (Hq / kv_heads).  The cache is read once, split evenly over the SMs whatever the
  * lengths; parts of a sequence are joined through the workspace (zero-filled once when it is created, left so by every
- * call, not shared by calls that may overlap).
+ * call, not shared by calls that may overlap).  out may be q itself, if that is dense, and overlaps nothing else.
  */
 size_t mp_paged_attention_decode_workspace_bytes(void);
 int mp_paged_attention_decode(int dtype, const mp_head_rows* q, int B, int Hq, int D, const mp_paged_cache* cache,
@@ -799,7 +799,7 @@ int mp_paged_attention_decode(int dtype, const mp_head_rows* q, int B, int Hq, i
 /*
  * Causal attention within packed sequences: rows cu_seqlens[b] .. cu_seqlens[b+1] of q[T,Hq,D], k and v[T,Hkv,D] are
  * sequence b (int32 [B + 1], ascending, at most T), and its row i attends to its rows 0..i.  Rows of out[T,Hq,D] that
- * belong to no sequence are left as they are.
+ * belong to no sequence are left as they are.  out may be q itself, if that is dense, and overlaps nothing else.
  */
 int mp_attention_prefill(int dtype, const mp_head_rows* q, const mp_head_rows* k, const mp_head_rows* v, int T, int Hq,
                          int Hkv, int D, const void* cu_seqlens_i32, int B, float scale, void* out, int* index_word,

@@ -268,7 +268,8 @@ struct Planner {
     for (int k = 0; k < kSortedBatch / 32; ++k) n += max(0, tiles[k] - l);
     return __reduce_add_sync(0xffffffffu, n);
   }
-  __device__ __forceinline__ Planner(const PrefillParams& params, int lane_) : p(params), lane(lane_), rows(params.pair_heads ? kTile : 2 * kTile) {
+  __device__ __forceinline__ Planner(const PrefillParams& params, int lane_)
+      : p(params), lane(lane_), rows(params.pair_heads ? kTile : 2 * kTile) {
     total = p.slots;
     level = 0;
     if (p.batch > kSortedBatch) return;
@@ -345,7 +346,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const uint32_t q_tile = smem_u32(smem), ring = q_tile + 2 * C::kTileBytes;
   const uint32_t kv_full = smem_u32(bars), kv_empty = kv_full + 8 * C::kStages, q_full = kv_empty + 8 * C::kStages,
                  q_empty = q_full + 16, s_full = q_empty + 16 /* [tile][part of the step] */, p_ready = s_full + 32 /* the same */,
-                 o_done = p_ready + 32 /* the same */, scanned = o_done + 32, s_read = scanned + 16, work_full = s_read + 16, work_empty = work_full + 8 * kAhead;
+                 o_done = p_ready + 32 /* the same */, scanned = o_done + 32, s_read = scanned + 16,
+                 work_full = s_read + 16, work_empty = work_full + 8 * kAhead;
   constexpr int kBars = 2 * C::kStages + 20 + 2 * kAhead;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);

@@ -724,7 +724,8 @@ def rotary_append_paged(q, k, v, cos_sin, positions, slots, k_cache, v_cache, *,
     ``(2i, 2i + 1)``.  Token ``t`` goes to offset ``slots[t] % page_size`` of page ``slots[t] // page_size`` of
     ``k_cache`` / ``v_cache [pages, Hkv, page_size, D]`` (views with other strides included), or nowhere where
     ``slots[t] < 0`` (padding); a slot may occur once per call (of two tokens with the same one, parts of either may be
-    stored).  ``positions`` and ``slots`` are int32 ``[T]``.  Inference only, as the attention operators: no gradients.
+    stored), and the tokens lie outside the cache.  ``positions`` and ``slots`` are int32 ``[T]``.  Inference only, as the
+    attention operators: no gradients.
 
     Returns ``(q_rotated, k_rotated | None)``; the caches are updated in place.  Positions and slots out of range touch no
     memory and raise at the next :func:`check_device_errors`.
@@ -742,7 +743,8 @@ def paged_attention_decode(q, k_cache, v_cache, page_table, seq_lens, *, scale: 
     ``q [B,Hq,D]`` fp16 or bf16, ``k_cache`` / ``v_cache [pages, Hkv, page_size, D]`` of the same type (``Hq`` a multiple of
     ``Hkv``), ``page_table`` int32 ``[B, pages of the longest]``, ``seq_lens`` int32 ``[B]``: tokens in the cache, the new
     one included; 0 gives a zero row.  What lies behind a sequence's end, in its last page and in its row of the table, is
-    never read.  ``scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``.  Nothing depends on lengths known to the host: a captured call
+    never read.  ``scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``, where that is contiguous.  Nothing depends on
+    lengths known to the host: a captured call
     serves whatever lengths the tensor holds at replay.  Pages and lengths out of range raise at the next
     :func:`check_device_errors`.
     """
