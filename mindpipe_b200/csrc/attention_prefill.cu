@@ -61,7 +61,8 @@ struct Prefill {
   static constexpr int kWeights = kApart ? 2 * (kTile + DP) : 0, kWeightStep = kApart ? kTile / 2 : kTile;
   static constexpr int kMultiplied = DP == 64 ? 1 : 2;         // of eight pairs of weights
   static constexpr int kBarBytes = 512;
-  static constexpr int kOutBytes = 8 * 32 * 128;               // 32 rows of 64 columns for each of eight warps
+  static constexpr int kOutColumns = DP / 2;
+  static constexpr int kOutBytes = 8 * 32 * 2 * kOutColumns;   // 32 rows of these for each of eight warps
   static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + kOutBytes + kBarBytes + 1024;
 };
 
@@ -772,34 +773,36 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       if (!wait_all(o_done + 16 * i + 8 * (C::kParts - 1), turn ^ 1)) { ok = false; break; }
       tcgen05_fence_after();
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      // 64 columns at a time through shared memory, so that a warp's stores are whole lines (a row to a thread took 3000 clocks
-      // of an item's end)
-      const uint32_t staged = ring + C::kStages * C::kTileBytes + ((warp - 4) * 32) * 128;
-      const int first_row = row_begin + quarter * 32;
-      char* dst = p.out + ((static_cast<long long>(seq_begin) + first_row) * p.q_heads + head) * p.dim * 2;
+      // Half a head's columns at a time through shared memory, so that a warp's stores are whole lines or sectors (a row to a
+      // thread took 3000 clocks of an item's end).  All of this code has to be fetched again when its turn comes, so a loop
+      // gains where rows are short: heads of 64 values by 64 columns 518 us, by 32 512; of 128 values by 64 41.4, by 32 42.0.
+      constexpr int kColumns = C::kOutColumns, kPieces = kColumns / 8;
+      const uint32_t staged = ring + C::kStages * C::kTileBytes + ((warp - 4) * 32) * (kColumns * 2);
+      const int first_row = row_begin + quarter * 32, own_row = lane / kPieces, piece = lane % kPieces;
+      char* dst = p.out + ((static_cast<long long>(seq_begin) + first_row + own_row) * p.q_heads + head) * p.dim * 2 + piece * 16;
+      const long long next_rows = static_cast<long long>(p.q_heads) * p.dim * (2 * 32 / kPieces);
 #pragma unroll 1
-      for (int c = 0; c < C::kBoxes; ++c) {
-        uint32_t o[2][32];
-        tmem_ld_32x32(o_tmem + 64 * c, o[0]);
-        tmem_ld_32x32(o_tmem + 64 * c + 32, o[1]);
-        tmem_ld_wait();
+      for (int c = 0; c < DP; c += kColumns) {
+        uint32_t o[kColumns / 32][32];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int x = 0; x < kColumns / 32; ++x) tmem_ld_32x32(o_tmem + c + 32 * x, o[x]);
+        tmem_ld_wait();
+        // (pieces of a row change places so that eight lanes write to all banks)
+#pragma unroll
+        for (int e = 0; e < kPieces; ++e) {
           uint32_t word[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x)
             word[x] = pack2<T>(__uint_as_float(o[e >> 2][(e & 3) * 8 + 2 * x]) * inv, __uint_as_float(o[e >> 2][(e & 3) * 8 + 2 * x + 1]) * inv);
-          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(staged + lane * 128 + ((e ^ (lane & 7)) << 4)), "r"(word[0]), "r"(word[1]),
-                       "r"(word[2]), "r"(word[3]) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(staged + lane * (kColumns * 2) + ((e ^ (lane * kPieces / 8 % kPieces)) << 4)),
+                       "r"(word[0]), "r"(word[1]), "r"(word[2]), "r"(word[3]) : "memory");
         }
         __syncwarp();
-        const int piece = lane & 7;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int r = e * 4 + (lane >> 3);
-          const uint4 v = lds16(staged + r * 128 + ((piece ^ (r & 7)) << 4));
-          if (first_row + r < len && c * 64 + piece * 8 < p.dim)
-            *reinterpret_cast<uint4*>(dst + (static_cast<long long>(r) * p.q_heads * p.dim + c * 64 + piece * 8) * 2) = v;
+        for (int e = 0; e < kPieces; ++e) {
+          const int r = e * (32 / kPieces) + own_row;
+          const uint4 v = lds16(staged + r * (kColumns * 2) + ((piece ^ (r * kPieces / 8 % kPieces)) << 4));
+          if (first_row + r < len && c + piece * 8 < p.dim) *reinterpret_cast<uint4*>(dst + e * next_rows + c * 2) = v;
         }
         __syncwarp();
       }
