@@ -743,7 +743,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 const int key = part * C::kPart + c + k;
-                if (key > row) continue;
+                const bool attends = key <= row;       // (by selection: 0 x NaN is not to be added)
                 const float weight = k ? pair.y : pair.x;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -753,11 +753,12 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                   for (int x = 0; x < 4; ++x) {
                     const float2 y = unpack2<T>(words[x]);
                     uint32_t &o0 = o[e * 8 + 2 * x], &o1 = o[e * 8 + 2 * x + 1];
-                    o0 = __float_as_uint(fmaf(weight, y.x, __uint_as_float(o0)));
-                    o1 = __float_as_uint(fmaf(weight, y.y, __uint_as_float(o1)));
+                    o0 = attends ? __float_as_uint(fmaf(weight, y.x, __uint_as_float(o0))) : o0;
+                    o1 = attends ? __float_as_uint(fmaf(weight, y.y, __uint_as_float(o1))) : o1;
                   }
                 }
               }
+              __syncwarp();                    // rows attend to different keys; all lanes are at the next load together
             }
             tmem_st_32x32(o_tmem + d0, o);
           }

@@ -1,0 +1,32 @@
+"""Values that are not finite, scales, ends out of order and operands that share memory, for the attention operators."""
+import pytest
+import torch
+
+from mindpipe_b200 import ops
+from tests import _attention_ref as ref
+from tests.test_attention_gpu import TYPES, heads
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 128), (3, 1, 64), (2, 2, 80)])
+@pytest.mark.parametrize("length", [50, 128, 250, 300])
+def test_prefill_values_that_are_not_finite_in_many_rows(length, h, hk, d, dtype):
+    """Every third token of a sequence has an infinite value in a column of its own: each row sees those of its own tokens."""
+    ends = [0, 13, 13 + length]
+    q, k, v = (x.contiguous() for x in heads(ends[-1], h, hk, d, dtype, length))
+    clean, hit = v.clone(), torch.zeros(ends[-1], h, d, dtype=torch.bool, device="cuda")
+    for n, token in enumerate(range(ends[1], ends[2], 3)):
+        column = 7 * n % d
+        v[token, :, column], clean[token, :, column] = float("inf"), 0
+        hit[token:ends[2], :, column] = True
+    got = ops.attention_prefill(q, k, v, i32(*ends))
+    want, tol = ref.prefill(q, k, clean, ends)
+    ref.assert_close(got[~hit], want[~hit], tol[~hit])
+    assert (got[hit] == float("inf")).all()
+    ops.check_device_errors()
