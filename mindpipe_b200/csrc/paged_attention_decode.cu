@@ -366,13 +366,21 @@ __global__ void __launch_bounds__(Decode<T, DP, HALF, EIGHTS, WHOLE>::kThreads, 
         for (int q = 0; q < kNQ; ++q) {
           const float inv0 = sum[q][0] == 0.0f ? 0.0f : 1.0f / sum[q][0], inv1 = sum[q][1] == 0.0f ? 0.0f : 1.0f / sum[q][1];
           char* dst = row_of(now, item, q * 8 + row0);
+          // (all exchanges in front of the stores, which not all lanes have)
+          uint32_t v[kMT][2];
 #pragma unroll
           for (int i = 0; i < kMT; ++i)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {      // eight columns by eight queries, to a query a lane's four
-              const uint32_t v = transpose(pack2<T>(o[i][q][2 * e] * inv0, o[i][q][2 * e + 1] * inv1));
-              if (q * 8 + row0 < rows && i * 16 + e * 8 < p.dim) *reinterpret_cast<uint32_t*>(dst + (i * 16 + e * 8 + col0) * 2) = v;
-            }
+            for (int e = 0; e < 2; ++e)        // eight columns by eight queries, to a query a lane's four
+              v[i][e] = transpose(pack2<T>(o[i][q][2 * e] * inv0, o[i][q][2 * e + 1] * inv1));
+          if (q * 8 + row0 < rows) {
+#pragma unroll
+            for (int i = 0; i < kMT; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (i * 16 + e * 8 < p.dim) *reinterpret_cast<uint32_t*>(dst + (i * 16 + e * 8 + col0) * 2) = v[i][e];
+          }
+          __syncwarp();
         }
       } else if (running) {
         const int rows = rows_of(now.unit), all = steps_of(tiles_of(now.len));

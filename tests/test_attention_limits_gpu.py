@@ -4,7 +4,7 @@ import torch
 
 from mindpipe_b200 import ops
 from tests import _attention_ref as ref
-from tests.test_attention_gpu import TYPES, heads
+from tests.test_attention_gpu import TYPES, heads, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -29,4 +29,15 @@ def test_prefill_values_that_are_not_finite_in_many_rows(length, h, hk, d, dtype
     want, tol = ref.prefill(q, k, clean, ends)
     ref.assert_close(got[~hit], want[~hit], tol[~hit])
     assert (got[hit] == float("inf")).all()
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("h,hk,d", [(9, 3, 72), (5, 1, 24), (14, 2, 128), (33, 3, 56), (26, 2, 120)])
+def test_decode_short_sequences_with_odd_groups_and_heads(h, hk, d, dtype):
+    """A warp alone, with fewer rows than the eight or sixteen of a tile: only some of its lanes have results to store."""
+    lens = [(13 * i) % 125 + 1 for i in range(320)]
+    args = paged(lens, h, hk, d, 16, dtype, seed=d)
+    want, tol = ref.decode(*args[:4], lens)
+    ref.assert_close(ops.paged_attention_decode(*args), want, tol)
     ops.check_device_errors()
