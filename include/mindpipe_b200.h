@@ -799,7 +799,7 @@ int mp_paged_attention_decode(int dtype, const mp_head_rows* q, int B, int Hq, i
 /*
  * Causal attention within packed sequences: rows cu_seqlens[b] .. cu_seqlens[b+1] of q[T,Hq,D], k and v[T,Hkv,D] are
  * sequence b (int32 [B + 1], ascending, at most T), and its row i attends to its rows 0..i.  Rows of out[T,Hq,D] that
- * belong to no sequence are left as they are.  out may be q itself, if that is dense, and overlaps nothing else.
+ * belong to no sequence are left as they are.  Where the ends are out of range or order, all of out is unspecified.  out may be q itself, if that is dense, and overlaps nothing else.
  */
 int mp_attention_prefill(int dtype, const mp_head_rows* q, const mp_head_rows* k, const mp_head_rows* v, int T, int Hq,
                          int Hkv, int D, const void* cu_seqlens_i32, int B, float scale, void* out, int* index_word,

@@ -263,6 +263,15 @@ struct Planner {
     len = good ? end - begin : 0;
     return good;
   }
+  // Not sorted, next() looks at the sequences that its search arrives at, which ends out of order mislead.  All of them are
+  // looked at when the block's last item is planned, a share by each block.
+  __device__ __forceinline__ void check_ends() const {
+    if (p.batch <= kSortedBatch) return;
+    for (long long b = static_cast<long long>(blockIdx.x) * 32 + lane; b < p.batch; b += gridDim.x * 32) {
+      int begin, len;
+      sequence(static_cast<int>(b), begin, len);
+    }
+  }
   __device__ __forceinline__ int beyond(int l) const {        // tiles with at least l in front of them
     int n = 0;
 #pragma unroll
@@ -589,6 +598,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         __syncwarp();
       }
+      plan.check_ends();
     }
   } else {
     // ---- one row of tile i to a thread

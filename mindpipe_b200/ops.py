@@ -761,7 +761,8 @@ def attention_prefill(q, k, v, cu_seqlens, *, scale: float | None = None, out=No
     ``q [T,Hq,D]``, ``k`` and ``v [T,Hkv,D]`` fp16 or bf16, strided views included, ``Hq`` a multiple of ``Hkv``;
     ``cu_seqlens`` int32 ``[B + 1]``, ascending, at most ``T``.  Returns ``out [T,Hq,D]``; rows that belong to no sequence
     are left as they are in ``out``, and unspecified without one.  ``scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``,
-    where that is contiguous.
+    where that is contiguous.  Ends out of range or order leave all of ``out`` unspecified and raise at the next
+    :func:`check_device_errors`.
     """
     device = _on_gpu(q, "q")
     y = _lib.host().attention_prefill(q, k, v, cu_seqlens, scale, out, _index_word(device), _error_word(device).data_ptr())

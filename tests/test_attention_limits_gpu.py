@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from mindpipe_b200 import ops
+from mindpipe_b200 import _lib, ops
 from tests import _attention_ref as ref
 from tests.test_attention_gpu import TYPES, heads, paged
 
@@ -40,4 +40,24 @@ def test_decode_short_sequences_with_odd_groups_and_heads(h, hk, d, dtype):
     args = paged(lens, h, hk, d, 16, dtype, seed=d)
     want, tol = ref.decode(*args[:4], lens)
     ref.assert_close(ops.paged_attention_decode(*args), want, tol)
+    ops.check_device_errors()
+
+
+@pytest.mark.parametrize("sequences", [257, 300, 5000])
+@pytest.mark.parametrize("h,hk", [(2, 1), (3, 3)])
+def test_prefill_one_end_out_of_order_among_many(sequences, h, hk):
+    """Beyond the number of sequences that are sorted, too: wherever the end is, and whichever way it is off."""
+    t = 20 * sequences
+    q, k, v = heads(t, h, hk, 64, torch.float16, 1)
+    good = list(range(0, t + 1, 20))
+    ops.attention_prefill(q, k, v, i32(*good))
+    ops.check_device_errors()
+    for at in (0, 1, sequences // 2, sequences - 1, sequences):
+        for end in (-1, 0, t, t + 1):
+            ends = good[:at] + [end] + good[at + 1:]
+            if ends == good or (end == 0 and at <= 1) or (end == t and at >= sequences - 1):
+                continue                                          # still ascending
+            ops.attention_prefill(q, k, v, i32(*ends))
+            with pytest.raises(_lib.MindPipeKernelError, match="out of range"):
+                ops.check_device_errors()
     ops.check_device_errors()
