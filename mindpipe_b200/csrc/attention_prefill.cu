@@ -783,7 +783,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       // ---- the row's result
       if (!wait_all(o_done + 16 * i + 8 * (C::kParts - 1), turn ^ 1)) { ok = false; break; }
       tcgen05_fence_after();
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float inv = 1.0f / sum;            // (0 where no score is above minus infinity: the row becomes 0 x infinity, NaN)
       // Half a head's columns at a time through shared memory, so that a warp's stores are whole lines or sectors (a row to a
       // thread took 3000 clocks of an item's end).  All of this code has to be fetched again when its turn comes, so a loop
       // gains where rows are short: heads of 64 values by 64 columns 518 us, by 32 512; of 128 values by 64 41.4, by 32 42.0.

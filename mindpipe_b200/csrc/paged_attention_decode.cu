@@ -336,8 +336,10 @@ __global__ void __launch_bounds__(Decode<T, DP, HALF, EIGHTS, WHOLE>::kThreads, 
   auto row_of = [&](const Cursor& c, int item, int row) {
     return p.out + (static_cast<long long>(c.seq) * p.q_heads + first_row(item) + row) * p.dim * 2;
   };
+  // An empty sequence gives zeros; one whose scores are all minus infinity has a sum of 0 too, and gives 0 x infinity, NaN.
+  auto inverse = [&](const Cursor& c, float sum) { return c.len == 0 ? 0.0f : 1.0f / sum; };
   auto store = [&](const Cursor& c, int row, int col, float4 v, float sum) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = inverse(c, sum);
     *reinterpret_cast<uint2*>(row_of(c, c.unit, row) + col * 2) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
   };
   auto team_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kTeam) : "memory"); };
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(Decode<T, DP, HALF, EIGHTS, WHOLE>::kThreads, 
         const int item = item_of(now), rows = rows_of(item);
 #pragma unroll
         for (int q = 0; q < kNQ; ++q) {
-          const float inv0 = sum[q][0] == 0.0f ? 0.0f : 1.0f / sum[q][0], inv1 = sum[q][1] == 0.0f ? 0.0f : 1.0f / sum[q][1];
+          const float inv0 = inverse(now, sum[q][0]), inv1 = inverse(now, sum[q][1]);
           char* dst = row_of(now, item, q * 8 + row0);
           // (all exchanges in front of the stores, which not all lanes have)
           uint32_t v[kMT][2];

@@ -61,3 +61,34 @@ def test_prefill_one_end_out_of_order_among_many(sequences, h, hk):
             with pytest.raises(_lib.MindPipeKernelError, match="out of range"):
                 ops.check_device_errors()
     ops.check_device_errors()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_of_minus_infinity_are_not_numbers(d):
+    """A softmax over scores that are all minus infinity is 0 / 0; one finite score among them takes all the weight."""
+    h, hk, n, page = 4, 2, 300, 16
+    q, k, v = (x.contiguous() for x in heads(n, h, hk, d, torch.bfloat16, d))
+    q[..., 0] = 1.0
+    k[:, 0], k[:, 0, 0] = 0, -float("inf")                        # every score of the first two heads
+    k[140, 0, 0] = 0.0                                            # ... but this token's, 0
+    out = ops.attention_prefill(q, k, v, i32(0, n))
+    assert out[:140, :2].isnan().all()
+    assert torch.equal(out[140:, :2], v[140, 0].expand(n - 140, 2, d))
+    want, tol = ref.prefill(q[:, 2:], k[:, 1:], v[:, 1:], [0, n])
+    ref.assert_close(out[:, 2:], want, tol)
+    pages = -(-n // page)
+    kc, vc = (torch.zeros(pages, hk, page, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    for cache, x in ((kc, k), (vc, v)):
+        for t in range(n):
+            cache[t // page, :, t % page] = x[t]
+    rows = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    for lens, some in ((300, True), (130, False), (12, False), (0, None)):
+        for batch in (1, 200):                                    # cut over the SMs; and a warp alone for the short ones
+            out = ops.paged_attention_decode(q[:1].expand(batch, h, d).contiguous(), kc, vc, rows.expand(batch, -1).contiguous(),
+                                             torch.full((batch,), lens, dtype=torch.int32, device="cuda"))
+            if some is None:
+                assert not out.any()
+                continue
+            assert torch.equal(out[:, :2], v[140, 0].expand(batch, 2, d)) if some else out[:, :2].isnan().all()
+            assert out[:, 2:].isfinite().all()
+    ops.check_device_errors()
