@@ -28,6 +28,8 @@
 // What a row may not attend to must not reach it, whatever it holds: scores are replaced where masked, but 0 x NaN is NaN in
 // the product with V.  So before the last step of a tile's rows the group clears rows of V behind the sequence's end and
 // looks for values that are not finite; where there are any, the threads add that step's product up themselves.
+#include <limits>
+
 #include "attention.cuh"
 
 namespace mp {
@@ -894,7 +896,10 @@ extern "C" int mp_attention_prefill(int dtype, const mp_head_rows* q, const mp_h
   p.slots = T / (p.pair_heads ? kTile : 2 * kTile) + B;
   p.per_slot = p.pair_heads ? Hq / 2 : Hq;
   if (static_cast<long long>(p.slots) * p.per_slot > 0x7fff0000LL) return MP_ERR_UNSUPPORTED;
-  p.scale_log2 = fmaxf(fabsf(scale) * attn::kLog2e, 1e-30f);      // masked scores stay minus infinity with a scale of 0 too
+  // Masked scores, minus infinity, are multiplied too: a scale of 0 becomes the smallest number above it, with which no finite
+  // score exceeds 2^-21.  A NaN stays one.
+  const float size = fabsf(scale) * attn::kLog2e;
+  p.scale_log2 = size == 0.0f ? std::numeric_limits<float>::denorm_min() : size;
   p.negate = scale < 0.0f ? 1u << 13 : 0u;
   CUtensorMap mq, mk, mv;
   if ((rc = head_map(&mq, dtype, qr, T, Hq, D, &p.q_order)) || (rc = head_map(&mk, dtype, kr, T, Hkv, D, &p.k_order)) ||

@@ -92,3 +92,21 @@ def test_rows_of_minus_infinity_are_not_numbers(d):
             assert torch.equal(out[:, :2], v[140, 0].expand(batch, 2, d)) if some else out[:, :2].isnan().all()
             assert out[:, 2:].isfinite().all()
     ops.check_device_errors()
+
+
+def test_a_scale_of_zero_is_zero_and_one_that_is_not_a_number_stays_so():
+    """With scores near the largest of fp32 too: all weights are equal, and a tiny scale counts as what it is."""
+    n, h, hk, d = 200, 2, 1, 64
+    q, k, v = (x.contiguous() for x in heads(n, h, hk, d, torch.bfloat16, 5))
+    q[..., 0], q[..., 1:], k[..., 1:] = 1e19, 0, 0
+    k[:, 0, 0] = torch.where(torch.arange(n, device="cuda") % 2 == 0, 1e19, -1e19).bfloat16()     # scores of 1e38 and -1e38
+    cu, page = i32(0, n), 8
+    kc, vc = (x.view(n // page, page, hk, d).transpose(1, 2) for x in (k, v))
+    rows, one = torch.arange(n // page, dtype=torch.int32, device="cuda")[None], i32(n)
+    for scale in (0.0, -0.0, 1e-38, -1e-38, 1e-33):
+        want, tol = ref.prefill(q, k, v, [0, n], scale)
+        ref.assert_close(ops.attention_prefill(q, k, v, cu, scale=scale), want, tol)
+        ref.assert_close(ops.paged_attention_decode(q[n - 1:], kc, vc, rows, one, scale=scale), want[n - 1:], tol[n - 1:])
+    assert ops.attention_prefill(q, k, v, cu, scale=float("nan")).isnan().all()
+    assert ops.paged_attention_decode(q[n - 1:], kc, vc, rows, one, scale=float("nan")).isnan().all()
+    ops.check_device_errors()
