@@ -790,6 +790,8 @@ int mp_rotary_append_paged(int dtype, const mp_head_rows* q, const mp_head_rows*
  * attends to the keys of head i / (Hq / kv_heads).  The cache is read once, split evenly over the SMs whatever the
  * lengths; parts of a sequence are joined through the workspace (zero-filled once when it is created, left so by every
  * call, not shared by calls that may overlap).  out may be q itself, if that is dense, and overlaps nothing else.
+ * Where ceil(B / 256) neighbouring sequences have some 2^29 tokens times kv_heads * ceil(Hq / kv_heads / 16) or more, the
+ * lengths may count as out of range, and then no row of out is written.
  */
 size_t mp_paged_attention_decode_workspace_bytes(void);
 int mp_paged_attention_decode(int dtype, const mp_head_rows* q, int B, int Hq, int D, const mp_paged_cache* cache,

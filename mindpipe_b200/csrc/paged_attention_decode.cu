@@ -154,7 +154,8 @@ __global__ void __launch_bounds__(Decode<T, DP, HALF, EIGHTS, WHOLE>::kThreads, 
   }
   s_scan[threadIdx.x] = sum_cost;
   if (lane == 31) s_warp[warp] = sum_cost;
-  // sums have 32 bits: a slice of 2^23 steps -- half a billion tokens -- is refused (with pages that are named many times)
+  // Sums have 32 bits: a slice with 2^23 steps over all its items is refused, and nothing is written.  With teams of four that
+  // is half a billion tokens times items: 67 million tokens of eight heads of keys (137 GB of them with 128 values).
   if (__syncthreads_or(about > 8388607.0f)) {
     if (p.index_word) *p.index_word = kBadIndex;
     return;

@@ -746,7 +746,8 @@ def paged_attention_decode(q, k_cache, v_cache, page_table, seq_lens, *, scale: 
     never read.  ``scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``, where that is contiguous.  Nothing depends on
     lengths known to the host: a captured call
     serves whatever lengths the tensor holds at replay.  Pages and lengths out of range raise at the next
-    :func:`check_device_errors`.
+    :func:`check_device_errors`; so may lengths that add up to half a billion tokens times ``Hkv`` (times sixteens of queries
+    to a head of keys) within ``ceil(B / 256)`` neighbouring sequences, and then no row of the result is written.
     """
     word = _index_word(_on_gpu(q, "q"))
     y = _lib.host().paged_decode(q, k_cache, v_cache, page_table, seq_lens, scale, out, word)

@@ -110,3 +110,22 @@ def test_a_scale_of_zero_is_zero_and_one_that_is_not_a_number_stays_so():
     assert ops.attention_prefill(q, k, v, cu, scale=float("nan")).isnan().all()
     assert ops.paged_attention_decode(q[n - 1:], kc, vc, rows, one, scale=float("nan")).isnan().all()
     ops.check_device_errors()
+
+
+@pytest.mark.parametrize("h", [16, 32])
+def test_decode_lists_beyond_32_bits_write_nothing(h):
+    """2^25 tokens and 16 heads of keys (or 16 and twice as many queries) are within the limit, 2^27 are beyond it; one page
+    stands for all of them."""
+    page, hk, d = 8192, 16, 8
+    kc = torch.zeros(1, hk, page, d, dtype=torch.float16, device="cuda")
+    vc = torch.ones_like(kc)
+    q = torch.zeros(2, h, d, dtype=torch.float16, device="cuda")
+    rows = torch.zeros(2, (1 << 27) // page, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 7.0)
+    ops.paged_attention_decode(q, kc, vc, rows, i32(5, 1 << 27), out=out)
+    with pytest.raises(_lib.MindPipeKernelError, match="out of range"):
+        ops.check_device_errors()
+    assert (out == 7).all()
+    ops.paged_attention_decode(q, kc, vc, rows, i32(5, 1 << 25), out=out)
+    assert (out == 1).all()                                       # (all values are 1, all weights equal)
+    ops.check_device_errors()
