@@ -777,7 +777,8 @@ typedef struct {
  * then their sines.  Pairs are (i, i + rotated / 2), or (2i, 2i + 1) with interleaved != 0; arithmetic in fp32, one
  * rounding.  q_out [T,Hq,D] and, unless null, k_out [T,Hkv,D] get the rotated queries and keys.  2 <= rotated <= D, even.
  * A token with a negative slot may have any position; one out of range then counts as 0.  Slots that occur twice
- * in a call are left with values of either token.  q_out and k_out may not overlap the inputs, nor these the cache.
+ * in a call are left with values of either token.  q_out and k_out may not overlap the inputs, nor these the
+ * cache, nor its entries one another.
  */
 int mp_rotary_append_paged(int dtype, const mp_head_rows* q, const mp_head_rows* k, const mp_head_rows* v,
                            const void* cos_sin_f32, int max_positions, int rotated, int interleaved,

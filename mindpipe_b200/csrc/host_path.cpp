@@ -22,6 +22,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <map>
 #include <memory>
@@ -667,6 +668,75 @@ bool apart(const at::Tensor& a, const at::Tensor& b) {
   const auto x = span_of(a), y = span_of(b);
   return x.second <= y.first || y.second <= x.first;
 }
+// Whether two 16-bit operands share memory, or a cache's entries with one another, where spans alone do not tell (the halves of
+// an interleaved pool): is there a sum of strides, each as often as the operands' sizes allow, that leads from one to the
+// other?  Strides and starts are multiples of 16 bytes, and pieces of 16 bytes are counted.  Largest stride first, what the
+// rest can still reach leaves two or three choices for each; a layout that leaves too many counts as sharing.
+struct Reach {
+  struct Step {
+    int64_t stride, least, most;             // pieces, and how often
+  };
+  c10::SmallVector<Step, 8> steps;
+  int budget = 20000;
+
+  void add(const at::Tensor& t, bool forward, bool back) {
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      const bool last = i + 1 == t.dim();
+      const int64_t n = last ? t.size(i) / 8 : t.size(i), stride = last ? 1 : t.stride(i) / 8;
+      if (n <= 1) continue;
+      Step* same = nullptr;
+      if (forward != back)
+        for (Step& s : steps)
+          if (s.stride == stride) same = &s;
+      if (!same) {
+        steps.push_back(Step{stride, 0, 0});
+        same = &steps.back();
+      }
+      if (forward) same->most += n - 1;
+      if (back) same->least -= n - 1;
+    }
+  }
+  void order() {
+    std::sort(steps.begin(), steps.end(), [](const Step& a, const Step& b) { return a.stride > b.stride; });
+  }
+  // `moved`: some step has been taken, or none has to be
+  bool leads(size_t from, int64_t way, bool moved) {
+    if (from == steps.size()) return way == 0 && moved;
+    if (--budget < 0) return true;
+    int64_t low = 0, high = 0;               // what the smaller strides reach
+    for (size_t i = from + 1; i < steps.size(); ++i) {
+      low += steps[i].least * steps[i].stride;
+      high += steps[i].most * steps[i].stride;
+    }
+    const Step s = steps[from];
+    if (s.stride == 0) return way == 0;
+    auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t first = std::max(s.least, -floor_div(high - way, s.stride)), last = std::min(s.most, floor_div(way - low, s.stride));
+    for (int64_t n = first; n <= last; ++n)
+      if (leads(from + 1, way - n * s.stride, moved || n != 0)) return true;
+    return false;
+  }
+};
+bool share(const at::Tensor& a, const at::Tensor& b) {
+  if (apart(a, b)) return false;
+  Reach r;
+  r.add(a, true, false);
+  r.add(b, false, true);
+  r.order();
+  return r.leads(0, (reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr())) / 16, true);
+}
+bool entries_share(const at::Tensor& t) {
+  Reach r;
+  r.add(t, true, true);
+  r.order();
+  int64_t inner = 0;                         // nested strides, as nearly always
+  bool nested = true;
+  for (auto s = r.steps.rbegin(); s != r.steps.rend(); ++s) {
+    nested = nested && s->stride > inner;
+    inner += s->most * s->stride;
+  }
+  return !nested && r.leads(0, 0, false);
+}
 // Results may replace the queries (a tile's or an item's are read before its result is written, and by nobody else), but be
 // nothing else that a call reads.
 bool output_apart(AttentionCall& call, const at::Tensor& out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
@@ -690,13 +760,13 @@ PyObject* rotary_append(PyObject*, PyObject* args) {
       !call.dense(to, "cos_sin", &table, 2, at::kFloat) || !call.dense(po, "positions", &pos, 1, at::kInt) ||
       !call.dense(so, "slots", &slots, 1, at::kInt) || !cache_arg(call, kco, vco, &kc, &vc, &cache))
     return nullptr;
-  if (kc->data_ptr() == vc->data_ptr()) return call.fail("k_cache and v_cache are the same memory"), nullptr;
-  for (int i = 0; i < 4; ++i)
-    if ((kc->size(i) > 1 && kc->stride(i) == 0) || (vc->size(i) > 1 && vc->stride(i) == 0))
-      return call.fail("the cache's entries share memory (an expanded tensor)"), nullptr;
   const int64_t t = q->size(0), d = q->size(2), rotated = table->size(1);
   if (k->sizes() != v->sizes() || k->size(0) != t || k->size(2) != d || k->size(1) != cache.kv_heads || kc->size(3) != d)
     return call.fail("q, k, v and cache shapes are inconsistent"), nullptr;
+  if (entries_share(*kc) || entries_share(*vc)) return call.fail("the cache's entries share memory (an expanded tensor)"), nullptr;
+  if (share(*kc, *vc)) return call.fail("k_cache and v_cache are the same memory, or overlap"), nullptr;
+  for (const at::Tensor* x : {q, k, v})
+    if (share(*x, *kc) || share(*x, *vc)) return call.fail("q, k or v overlaps the cache"), nullptr;
   if (pos->size(0) != t || slots->size(0) != t) return call.fail("positions and slots must have one entry per token"), nullptr;
   if (rotated < 2 || rotated % 2 || rotated > d || table->size(0) == 0 || reinterpret_cast<uintptr_t>(table->data_ptr()) % 16)
     return call.fail("cos_sin must be [positions, rotated], 16-byte aligned, with an even number of rotated values up to D"), nullptr;

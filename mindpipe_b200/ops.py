@@ -724,7 +724,7 @@ def rotary_append_paged(q, k, v, cos_sin, positions, slots, k_cache, v_cache, *,
     ``(2i, 2i + 1)``.  Token ``t`` goes to offset ``slots[t] % page_size`` of page ``slots[t] // page_size`` of
     ``k_cache`` / ``v_cache [pages, Hkv, page_size, D]`` (views with other strides included), or nowhere where
     ``slots[t] < 0`` (padding); a slot may occur once per call (of two tokens with the same one, parts of either may be
-    stored), and the tokens lie outside the cache.  ``positions`` and ``slots`` are int32 ``[T]``.  Inference only, as the
+    stored).  Views that share memory -- the two caches, a cache's entries, tokens within a cache -- raise ``ValueError``.  ``positions`` and ``slots`` are int32 ``[T]``.  Inference only, as the
     attention operators: no gradients.
 
     Returns ``(q_rotated, k_rotated | None)``; the caches are updated in place.  Positions and slots out of range touch no

@@ -129,3 +129,68 @@ def test_decode_lists_beyond_32_bits_write_nothing(h):
     ops.paged_attention_decode(q, kc, vc, rows, i32(5, 1 << 25), out=out)
     assert (out == 1).all()                                       # (all values are 1, all weights equal)
     ops.check_device_errors()
+
+
+def pieces(x, room):
+    """The 16-byte pieces of `room` that each entry of a tensor [..., D] covers."""
+    at = torch.arange(room.numel()).as_strided(x.shape, x.stride(), (x.data_ptr() - room.data_ptr()) // 2)
+    return (at[..., ::8] // 8).flatten().tolist()
+
+
+def append_of(q, k, v, kc, vc):
+    at = torch.arange(q.shape[0], dtype=torch.int32, device="cuda")
+    cs = torch.cat([torch.ones(8, 4), torch.zeros(8, 4)], 1).cuda()
+    return ops.rotary_append_paged(q, k, v, cs, at, at, kc, vc)
+
+
+def test_caches_of_one_memory_are_taken_where_their_entries_are_apart():
+    room = torch.zeros(6 * 2 * 4 * 8 * 16, dtype=torch.float16, device="cuda")
+    q, k, v = torch.zeros(3, 2, 4, 8, dtype=torch.float16, device="cuda").unbind()
+    dense, parts = room[:6 * 4 * 8 * 8].view(6, 4, 8, 8), room.view(6, 2, 4, 8, 16)
+    apart = [(parts[:, 0, ..., :8], parts[:, 1, ..., :8]),                    # a page of keys, a page of values
+             (parts[:, 0, ..., :8], parts[:, 0, ..., 8:]),                    # a key's values beside it
+             (parts[:, 0, ..., :8], parts[:, 1, ..., :8].reshape(6, 8, 4, 8).transpose(1, 2)),
+             (dense[:3], dense[3:]), (parts[::2, 0, ..., :8], parts[1::2, 0, ..., :8])]
+    for kc, vc in apart:
+        append_of(q, k, v, kc, vc)
+    shifted = room[8 * 8:8 * 8 + dense.numel()].view(6, 4, 8, 8)
+    for kc, vc in ((dense[:4], dense[2:]), (dense, shifted), (dense, dense.view(6, 8, 4, 8).transpose(1, 2)), (dense[::2], dense[:3])):
+        with pytest.raises(ValueError, match="overlap"):
+            append_of(q, k, v, kc, vc)
+    with pytest.raises(ValueError, match="share memory"):
+        append_of(q, k, v, room.as_strided((6, 4, 8, 8), (8 * 8, 8, 8, 1)), parts[:, 1, ..., :8])
+    kc, vc = parts[:, 0, ..., :8], parts[:, 1, ..., :8]
+    for i in range(3):
+        mine = [q, k, v]
+        mine[i] = kc[2, :, :4].transpose(0, 1)                    # the tokens' place is in the cache
+        with pytest.raises(ValueError, match="overlaps the cache"):
+            append_of(*(x[:2] for x in mine), kc, vc)
+    beside = parts[2, 0, :, :4, 8:].transpose(0, 1)[:2]           # between a cache's rows, not in it
+    append_of(beside, beside, beside, kc, vc)
+    ops.check_device_errors()
+
+
+def test_whether_random_views_share_memory_is_told_exactly():
+    import random
+    rng = random.Random(7)
+    room = torch.zeros(1 << 15, dtype=torch.float16, device="cuda")
+    q, k, v = torch.zeros(3, 1, 2, 8, dtype=torch.float16, device="cuda").unbind()
+    counts = {True: 0, False: 0}
+    for _ in range(3000):
+        shape = (rng.randint(1, 4), 2, rng.randint(1, 4), 8)
+        sides = []
+        for _ in range(2):
+            stride = [8 * rng.choice((1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64)) for _ in range(3)] + [1]
+            sides.append(room.as_strided(shape, stride, 8 * rng.randint(0, 40)))
+        if rng.random() < 0.6:
+            sides[1] = room.as_strided(shape, sides[0].stride(), 8 * rng.randint(0, 40))
+        one, two = (pieces(x, room) for x in sides)
+        shared = len(set(one)) < len(one) or len(set(two)) < len(two) or bool(set(one) & set(two))
+        counts[shared] += 1
+        if shared:
+            with pytest.raises(ValueError, match="memory"):
+                append_of(q, k, v, *sides)
+        else:
+            append_of(q, k, v, *sides)
+    assert min(counts.values()) > 200
+    ops.check_device_errors()
