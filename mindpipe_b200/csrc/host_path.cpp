@@ -767,6 +767,7 @@ PyObject* rotary_append(PyObject*, PyObject* args) {
   if (share(*kc, *vc)) return call.fail("k_cache and v_cache are the same memory, or overlap"), nullptr;
   for (const at::Tensor* x : {q, k, v})
     if (share(*x, *kc) || share(*x, *vc)) return call.fail("q, k or v overlaps the cache"), nullptr;
+  if (q->size(1) == 0) return call.fail("q has no heads"), nullptr;
   if (pos->size(0) != t || slots->size(0) != t) return call.fail("positions and slots must have one entry per token"), nullptr;
   if (rotated < 2 || rotated % 2 || rotated > d || table->size(0) == 0 || reinterpret_cast<uintptr_t>(table->data_ptr()) % 16)
     return call.fail("cos_sin must be [positions, rotated], 16-byte aligned, with an even number of rotated values up to D"), nullptr;
@@ -774,7 +775,7 @@ PyObject* rotary_append(PyObject*, PyObject* args) {
   at::Tensor q_out = dense_like(*q), k_out;
   if (want_k) k_out = dense_like(*k);
   int rc = MP_OK;
-  if (t && q->size(1)) {
+  if (t) {
     const mp_head_rows qr = head_rows(*q), kr = head_rows(*k), vr = head_rows(*v);
     rc = mp_rotary_append_paged(call.type(), &qr, &kr, &vr, table->data_ptr(), static_cast<int>(table->size(0)),
                                 static_cast<int>(rotated), interleaved, pos->data_ptr(), slots->data_ptr(), static_cast<int>(t),

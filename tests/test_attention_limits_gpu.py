@@ -194,3 +194,11 @@ def test_whether_random_views_share_memory_is_told_exactly():
             append_of(q, k, v, *sides)
     assert min(counts.values()) > 200
     ops.check_device_errors()
+
+
+def test_append_without_query_heads_is_refused():
+    """(It would have to store keys and values all the same.)"""
+    k, v = torch.zeros(2, 3, 4, 8, dtype=torch.float16, device="cuda").unbind()
+    kc, vc = torch.zeros(2, 6, 4, 8, 8, dtype=torch.float16, device="cuda").unbind()
+    with pytest.raises(ValueError, match="no heads"):
+        append_of(k[:, :0], k, v, kc, vc)
