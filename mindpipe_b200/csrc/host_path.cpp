@@ -739,9 +739,11 @@ bool entries_share(const at::Tensor& t) {
 }
 // Results may replace the queries (a tile's or an item's are read before its result is written, and by nobody else), but be
 // nothing else that a call reads.
-bool output_apart(AttentionCall& call, const at::Tensor& out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
-  const bool same = out.data_ptr() == q.data_ptr() && q.is_contiguous();
-  if ((!same && !apart(out, q)) || !apart(out, k) || !apart(out, v))
+bool output_apart(AttentionCall& call, const at::Tensor& out, const at::Tensor& q,
+                  std::initializer_list<const at::Tensor*> others) {
+  bool ok = (out.data_ptr() == q.data_ptr() && q.is_contiguous()) || apart(out, q);
+  for (const at::Tensor* x : others) ok = ok && apart(out, *x);
+  if (!ok)
     return call.fail("out overlaps an operand (it may be q itself, where that is contiguous)");
   return true;
 }
@@ -808,7 +810,7 @@ PyObject* paged_decode(PyObject*, PyObject* args) {
   if (PyErr_Occurred()) return nullptr;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(call.device));
   at::Tensor out;
-  if (!output_arg(call, oo, *q, &out) || (oo != Py_None && !output_apart(call, out, *q, *kc, *vc))) return nullptr;
+  if (!output_arg(call, oo, *q, &out) || (oo != Py_None && !output_apart(call, out, *q, {kc, vc, table, lens}))) return nullptr;
   if (b && h) {
     const cudaStream_t st = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(call.device)).stream();
     const Scratch ws(mp_paged_attention_decode_workspace_bytes(), call.device, st, kAttention, true);
@@ -840,7 +842,7 @@ PyObject* attention_prefill(PyObject*, PyObject* args) {
   if (PyErr_Occurred()) return nullptr;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(call.device));
   at::Tensor out;
-  if (!output_arg(call, oo, *q, &out) || (oo != Py_None && !output_apart(call, out, *q, *k, *v))) return nullptr;
+  if (!output_arg(call, oo, *q, &out) || (oo != Py_None && !output_apart(call, out, *q, {k, v, cu}))) return nullptr;
   if (t && h && cu->size(0) > 1) {
     const mp_head_rows qr = head_rows(*q), kr = head_rows(*k), vr = head_rows(*v);
     const int rc = mp_attention_prefill(call.type(), &qr, &kr, &vr, static_cast<int>(t), static_cast<int>(h), static_cast<int>(hk),

@@ -202,3 +202,17 @@ def test_append_without_query_heads_is_refused():
     kc, vc = torch.zeros(2, 6, 4, 8, 8, dtype=torch.float16, device="cuda").unbind()
     with pytest.raises(ValueError, match="no heads"):
         append_of(k[:, :0], k, v, kc, vc)
+
+
+def test_results_over_index_tensors_are_refused():
+    room = torch.zeros(4, 4, 64, dtype=torch.float16, device="cuda")
+    index = room.view(-1).view(torch.int32)
+    q, k, v = torch.zeros(3, 4, 4, 64, dtype=torch.float16, device="cuda").unbind()
+    kc, vc = torch.zeros(2, 4, 4, 16, 64, dtype=torch.float16, device="cuda").unbind()
+    rows, n = torch.zeros(4, 1, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    for call in (lambda: ops.paged_attention_decode(q, kc, vc, index[:4].view(4, 1), n, out=room),
+                 lambda: ops.paged_attention_decode(q, kc, vc, rows, index[-4:], out=room),
+                 lambda: ops.attention_prefill(q, k, v, index[:2], out=room)):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+    ops.check_device_errors()
