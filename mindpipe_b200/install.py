@@ -199,8 +199,11 @@ def install_paged_attention(model: nn.Module, cache: PagedKVCache, *, cos_sin: t
                 raise ValueError(f"{name}: {extra} is not part of the paged attention")
         if getattr(attn, "is_causal", True) is False:
             raise ValueError(f"{name}: the paged attention is causal")
+        # (one that is installed already moves to this cache with its own scale and pairs)
+        again = isinstance(attn, PagedSelfAttention)
         made.append((layer, name, PagedSelfAttention(attn, cache, i, cos_sin, head_dim=getattr(attn, "head_dim", None),
-                                                     scale=getattr(attn, "scaling", None))))
+                                                     scale=attn.scale if again else getattr(attn, "scaling", None),
+                                                     interleaved=again and attn.interleaved)))
     for layer, _, new in made:
         layer.self_attn = new
     return [name for _, name, _ in made]
