@@ -35,17 +35,22 @@ _ATTN_PROJ = ("q_proj", "k_proj", "v_proj")
 _MLP_PROJ = ("gate_proj", "up_proj", "down_proj")
 
 
-def get_blocks(model: nn.Module):
-    """The decoder layers, found the way ``awq/quantize/pre_quant.py:47-76`` finds them (text backbones only)."""
+def _backbone(model: nn.Module) -> nn.Module:
+    """The module that holds the decoder layers, found the way ``awq/quantize/pre_quant.py:47-76`` finds them."""
     if hasattr(model, "model") and hasattr(model.model, "language_model"):
-        return model.model.language_model.layers
+        return model.model.language_model
     if hasattr(model, "language_model") and hasattr(model.language_model, "layers"):
-        return model.language_model.layers
+        return model.language_model
     if hasattr(model, "model") and hasattr(model.model, "layers"):
-        return model.model.layers
+        return model.model
     if hasattr(model, "layers") and isinstance(model.layers, (nn.ModuleList, list)):
-        return model.layers
+        return model
     raise NotImplementedError(type(model))
+
+
+def get_blocks(model: nn.Module):
+    """The decoder layers (text backbones only)."""
+    return _backbone(model).layers
 
 
 def _blocks_prefix(model: nn.Module) -> str:
@@ -168,27 +173,19 @@ def install_paged_attention(model: nn.Module, cache: PagedKVCache, *, cos_sin: t
     """Run the attention of every decoder layer on ``cache``; returns the qualified names that were replaced.
 
     Works before or after the installers of the linears; ``install_paged_attention`` does not touch them.  The rotation's
-    table is ``cos_sin`` (fp32 ``[positions, rotated]``, cosines then sines) or made from the model's ``rotary_emb``
+    table is ``cos_sin`` (fp32 ``[positions, rotated]``, cosines then sines) or made from the ``rotary_emb`` beside the layers
     (``inv_freq`` and ``attention_scaling``) for ``max_positions`` positions (default: the config's
     ``max_position_embeddings``).  Layers whose attention does more than project, rotate and attend -- normalised
     queries or keys, sliding windows, capped scores -- or look ahead raise ``ValueError`` before anything is replaced.  The
     rotation pairs value ``i`` of a head with ``i + rotated / 2``; a model that pairs neighbours is put together from
     :class:`PagedSelfAttention` with ``interleaved=True``.
     """
-    layers, prefix = get_blocks(model), _blocks_prefix(model)
+    backbone, prefix = _backbone(model), _blocks_prefix(model)
+    layers = backbone.layers
     if len(layers) != cache.pool.shape[0]:
         raise ValueError(f"the model has {len(layers)} layers, the cache {cache.pool.shape[0]}")
     if cos_sin is None:
-        rotary = next((m for m in model.modules() if hasattr(m, "inv_freq")), None)
-        if rotary is None:
-            raise ValueError("the model has no rotary_emb with inv_freq: pass cos_sin")
-        kind = getattr(rotary, "rope_type", "default")
-        if kind in ("dynamic", "longrope"):
-            raise ValueError(f"the frequencies of rope type {kind!r} depend on the length: pass cos_sin")
-        limit = max_positions or getattr(getattr(model, "config", None), "max_position_embeddings", None)
-        if limit is None:
-            raise ValueError("pass max_positions")
-        cos_sin = rotary_table(rotary.inv_freq.to(cache.pool.device), int(limit), float(getattr(rotary, "attention_scaling", 1.0)))
+        cos_sin = _model_table(model, backbone, max_positions, cache.pool.device)
     made = []
     for i, layer in enumerate(layers):
         attn, name = getattr(layer, "self_attn", None), f"{prefix}.{i}.self_attn"
@@ -207,6 +204,24 @@ def install_paged_attention(model: nn.Module, cache: PagedKVCache, *, cos_sin: t
     for layer, _, new in made:
         layer.self_attn = new
     return [name for _, name, _ in made]
+
+
+def _model_table(model: nn.Module, backbone: nn.Module, max_positions: int | None, device) -> torch.Tensor:
+    """The table of the rotary module that serves ``backbone`` (a vision tower beside it may have one of its own)."""
+    rotary = [m for m in backbone.modules() if hasattr(m, "inv_freq")] or [m for m in model.children() if hasattr(m, "inv_freq")]
+    if not rotary:
+        raise ValueError("the model has no rotary_emb with inv_freq: pass cos_sin")
+    for m in rotary:
+        kind = getattr(m, "rope_type", "default")
+        if kind in ("dynamic", "longrope"):
+            raise ValueError(f"the frequencies of rope type {kind!r} depend on the length: pass cos_sin")
+        if not torch.equal(m.inv_freq.to(rotary[0].inv_freq.device), rotary[0].inv_freq):
+            raise ValueError("the model's layers rotate by different frequencies")
+    limit = max_positions or next((n for n in (getattr(getattr(m, "config", None), "max_position_embeddings", None) for m in (backbone, model))
+                                   if n is not None), None)
+    if limit is None:
+        raise ValueError("pass max_positions")
+    return rotary_table(rotary[0].inv_freq.to(device), int(limit), float(getattr(rotary[0], "attention_scaling", 1.0)))
 
 
 _W4_KEYS = ("weight_packed", "weight_scale", "weight_zero_point", "weight_shape", "bias")

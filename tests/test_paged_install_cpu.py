@@ -25,3 +25,33 @@ def test_installing_again_keeps_scale_and_pairs():
     first, second = (layer.self_attn for layer in model.model.layers)
     assert first.scale == 0.25 and first.interleaved is False and second.scale is None and second.interleaved is True
     assert first.cache is cache and first.q_proj is attn.q_proj and isinstance(first, PagedSelfAttention)
+
+
+class _Rotary(nn.Module):
+    def __init__(self, inv_freq):
+        super().__init__()
+        self.register_buffer("inv_freq", inv_freq)
+
+
+def test_the_table_is_that_of_the_layers_rotation():
+    """A tower beside the language model, in front of it in the tree, has frequencies of its own."""
+    class Tree(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.model = nn.Module()
+            self.model.visual = _Rotary(torch.ones(4))
+            self.model.language_model = TinyLlama().model
+            self.model.language_model.rotary_emb = _Rotary(inv)
+
+    inv = 100.0 ** (-torch.arange(32) / 32)
+    model = Tree()
+    install.install_paged_attention(model, make_cache(), max_positions=50)
+    assert torch.equal(model.model.language_model.layers[1].self_attn.cos_sin, rotary_table(inv, 50))
+    model = Tree()
+    del model.model.language_model.rotary_emb
+    with pytest.raises(ValueError, match="pass cos_sin"):
+        install.install_paged_attention(model, make_cache(), max_positions=50)
+    model = Tree()
+    model.model.language_model.layers[1].rotary_emb = _Rotary(inv * 2)
+    with pytest.raises(ValueError, match="different frequencies"):
+        install.install_paged_attention(model, make_cache(), max_positions=50)
