@@ -29,6 +29,7 @@ import torch
 from torch import nn
 
 from .attention import PagedKVCache, PagedSelfAttention, rotary_table
+from .attention_check import check_attention, check_config, check_table
 from .modules import SmoothQuantLinear, SmoothQuantPackedMoeExperts, VllmPackedInt4Linear
 
 _ATTN_PROJ = ("q_proj", "k_proj", "v_proj")
@@ -175,10 +176,11 @@ def install_paged_attention(model: nn.Module, cache: PagedKVCache, *, cos_sin: t
     Works before or after the installers of the linears; ``install_paged_attention`` does not touch them.  The rotation's
     table is ``cos_sin`` (fp32 ``[positions, rotated]``, cosines then sines) or made from the ``rotary_emb`` beside the layers
     (``inv_freq`` and ``attention_scaling``) for ``max_positions`` positions (default: the config's
-    ``max_position_embeddings``).  Layers whose attention does more than project, rotate and attend -- normalised
-    queries or keys, sliding windows, capped scores -- or look ahead raise ``ValueError`` before anything is replaced.  The
-    rotation pairs value ``i`` of a head with ``i + rotated / 2``; a model that pairs neighbours is put together from
-    :class:`PagedSelfAttention` with ``interleaved=True``.
+    ``max_position_embeddings``).  Layers whose attention does anything but project, rotate in halves and attend causally --
+    normalised queries or keys, windows smaller than the table, capped scores, clamped values, rotation of neighbours or none,
+    positions of several parts, whatever else changes its results (:mod:`mindpipe_b200.attention_check`) -- or that carry
+    another state from token to token raise ``ValueError`` before anything is replaced.  A model that pairs neighbours, or whose
+    attention cannot be asked, is put together from :class:`PagedSelfAttention` by hand.
     """
     backbone, prefix = _backbone(model), _blocks_prefix(model)
     layers = backbone.layers
@@ -191,16 +193,21 @@ def install_paged_attention(model: nn.Module, cache: PagedKVCache, *, cos_sin: t
         attn, name = getattr(layer, "self_attn", None), f"{prefix}.{i}.self_attn"
         if attn is None:
             raise ValueError(f"Unsupported layer layout at {prefix}.{i}: expected .self_attn")
+        config = next((c for c in (getattr(m, "config", None) for m in (attn, backbone, model)) if c is not None), None)
+        check_config(config, name, i, cos_sin.shape[0])
+        if isinstance(attn, PagedSelfAttention):                  # installed already: it keeps its own scale and pairs
+            made.append((layer, name, PagedSelfAttention(attn, cache, i, cos_sin, scale=attn.scale, interleaved=attn.interleaved)))
+            continue
         for extra in ("q_norm", "k_norm", "sliding_window", "attn_logit_softcapping", "sinks"):
             if getattr(attn, extra, None) is not None:
                 raise ValueError(f"{name}: {extra} is not part of the paged attention")
         if getattr(attn, "is_causal", True) is False:
             raise ValueError(f"{name}: the paged attention is causal")
-        # (one that is installed already moves to this cache with its own scale and pairs)
-        again = isinstance(attn, PagedSelfAttention)
-        made.append((layer, name, PagedSelfAttention(attn, cache, i, cos_sin, head_dim=getattr(attn, "head_dim", None),
-                                                     scale=attn.scale if again else getattr(attn, "scaling", None),
-                                                     interleaved=again and attn.interleaved)))
+        if any(isinstance(m, nn.Conv1d) for m in layer.modules()):
+            raise ValueError(f"{prefix}.{i}: a convolution over tokens has a state of its own, which the cache does not hold")
+        new = PagedSelfAttention(attn, cache, i, cos_sin, head_dim=getattr(attn, "head_dim", None), scale=getattr(attn, "scaling", None))
+        check_attention(attn, name, head_dim=new.head_dim, rotated=cos_sin.shape[1], scale=new.scale)
+        made.append((layer, name, new))
     for layer, _, new in made:
         layer.self_attn = new
     return [name for _, name, _ in made]
@@ -221,7 +228,9 @@ def _model_table(model: nn.Module, backbone: nn.Module, max_positions: int | Non
                                    if n is not None), None)
     if limit is None:
         raise ValueError("pass max_positions")
-    return rotary_table(rotary[0].inv_freq.to(device), int(limit), float(getattr(rotary[0], "attention_scaling", 1.0)))
+    table = rotary_table(rotary[0].inv_freq.to(device), int(limit), float(getattr(rotary[0], "attention_scaling", 1.0)))
+    check_table(rotary[0], table)
+    return table
 
 
 _W4_KEYS = ("weight_packed", "weight_scale", "weight_zero_point", "weight_shape", "bias")
