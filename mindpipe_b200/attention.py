@@ -213,7 +213,10 @@ class PagedSelfAttention(nn.Module):
 
     def _apply(self, fn, *args, **kwargs):
         table = self._buffers.pop("cos_sin")             # moved with the module, never cast
-        super()._apply(fn, *args, **kwargs)
+        try:
+            super()._apply(fn, *args, **kwargs)
+        finally:
+            self._buffers["cos_sin"] = table
         self._buffers["cos_sin"] = table.to(fn(torch.empty(0, dtype=torch.float32, device=table.device)).device)
         return self
 

@@ -235,3 +235,15 @@ def test_positions_of_several_parts_are_refused():
     for table in (None, rotary_table(torch.ones(32), 64)):
         with pytest.raises(ValueError, match="mrope_section|in halves|cannot be compared"):
             install.install_paged_attention(model, make_cache(2, 2, 64), cos_sin=table)
+
+
+def test_a_move_that_fails_leaves_the_table():
+    model = TinyLlama()
+    install.install_paged_attention(model, make_cache(), cos_sin=rotary_table(torch.ones(32), 8))
+    attn = model.model.layers[0].self_attn
+
+    def fails(t):
+        raise RuntimeError("out of memory")
+    with pytest.raises(RuntimeError):
+        attn._apply(fails)
+    assert attn.cos_sin.shape == (8, 64) and [n for n, _ in attn.named_buffers()] == ["cos_sin"]
