@@ -40,6 +40,8 @@ class Step:
     cu_seqlens: torch.Tensor | None = None   # int32 [sequences + 1]
     page_table: torch.Tensor | None = None   # int32 [sequences, pages]
     seq_lens: torch.Tensor | None = None     # int32 [sequences]
+    longest: int = 0                         # tokens of the longest sequence, as the host knows it; 0: it does not
+    positions_limit: int | None = None       # of the tables that forwards have used with this step
 
     @property
     def tokens(self) -> int:
@@ -58,7 +60,8 @@ class PagedKVCache:
             model(torch.cat([a, b])[None], position_ids=step.positions.long()[None], use_cache=False)
         step = cache.next_token(step.sequences)
 
-    The bookkeeping is host code; running out of pages raises ``RuntimeError`` and changes nothing.
+    The bookkeeping is host code; running out of pages raises ``RuntimeError`` and changes nothing.  A step with a sequence
+    longer than the rotation's table raises ``ValueError`` in the forward, before anything is stored.
     """
 
     def __init__(self, num_layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, *,
@@ -115,14 +118,14 @@ class PagedKVCache:
             positions.extend(range(n))
             slots.extend(own[i // self.page_size] * self.page_size + i % self.page_size for i in range(n))
             ends.append(ends[-1] + n)
-        return Step(ids, self._tensor(positions), self._tensor(slots), cu_seqlens=self._tensor(ends))
+        return Step(ids, self._tensor(positions), self._tensor(slots), cu_seqlens=self._tensor(ends), longest=max(lengths))
 
     def next_token(self, sequences, into: Step | None = None) -> Step:
         """One token more for each of the sequences.
 
         ``into``: an earlier step of as many sequences, whose tensors are written instead of new ones -- a captured forward
         then runs the new step when replayed.  Its table keeps its width: sequences that outgrow it raise ``ValueError``
-        (:meth:`reserve` makes a wider one)."""
+        (:meth:`reserve` makes a wider one), and so do sequences that outgrow the rotation's table of the forward."""
         sequences = list(sequences)
         if len(set(sequences)) != len(sequences):
             raise ValueError("a sequence may appear once in a step")
@@ -136,6 +139,9 @@ class PagedKVCache:
             if into.page_table.shape[1] < width:
                 raise ValueError(f"a sequence has {width} pages, the step's table room for {into.page_table.shape[1]}")
             width = into.page_table.shape[1]
+        longest = max(self._length[s] for s in sequences) + 1
+        if into is not None and into.positions_limit is not None and longest > into.positions_limit:
+            raise ValueError(f"a sequence has {longest} tokens, the rotation's table of the step's forwards {into.positions_limit} positions")
         for s, page in zip(grow, self._take(len(grow))):
             self._pages[s].append(page)
         positions, slots, lens, table = [], [], [], []
@@ -148,10 +154,10 @@ class PagedKVCache:
             table.append(self._pages[s] + [-1] * (width - len(self._pages[s])))
         if into is None:
             return Step(sequences, self._tensor(positions), self._tensor(slots), page_table=self._tensor(table),
-                        seq_lens=self._tensor(lens))
+                        seq_lens=self._tensor(lens), longest=longest)
         for name, values in (("positions", positions), ("slots", slots), ("page_table", table), ("seq_lens", lens)):
             getattr(into, name).copy_(torch.tensor(values, dtype=torch.int32))
-        into.sequences = sequences
+        into.sequences, into.longest = sequences, longest
         return into
 
     def reserve(self, batch: int, longest: int) -> Step:
@@ -229,6 +235,10 @@ class PagedSelfAttention(nn.Module):
         tokens = hidden_states.numel() // hidden_states.shape[-1]
         if tokens != step.tokens:
             raise ValueError(f"the running step has {step.tokens} tokens, the input {tokens}")
+        limit = self.cos_sin.shape[0]
+        if step.longest > limit:
+            raise ValueError(f"a sequence has {step.longest} tokens, the rotation's table {limit} positions")
+        step.positions_limit = limit if step.positions_limit is None else min(limit, step.positions_limit)
         x = hidden_states.reshape(tokens, -1)
         q, k, v = (proj(x).view(tokens, -1, self.head_dim) for proj in (self.q_proj, self.k_proj, self.v_proj))
         k_cache, v_cache = self.cache.layer(self.layer_idx)

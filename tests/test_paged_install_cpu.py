@@ -247,3 +247,35 @@ def test_a_move_that_fails_leaves_the_table():
     with pytest.raises(RuntimeError):
         attn._apply(fails)
     assert attn.cos_sin.shape == (8, 64) and [n for n, _ in attn.named_buffers()] == ["cos_sin"]
+
+
+def test_sequences_beyond_the_rotations_table_are_refused(monkeypatch):
+    """The kernels would store nothing of their tokens and say so at the next look for errors only."""
+    _attention_cpu.use(monkeypatch)
+    model, cache = TinyLlama().float(), make_cache()
+    install.install_paged_attention(model, cache, cos_sin=rotary_table(torch.ones(32), 8))
+    attn, x = model.model.layers[0].self_attn, torch.randn(40, 256)
+    cache.pool.zero_()
+    step = cache.prompts([9, 2])
+    with cache.running(step), pytest.raises(ValueError, match="8 positions"):
+        attn(x[:11])
+    assert not cache.pool.any()
+    step = cache.prompts([7, 8])
+    with cache.running(step):
+        attn(x[:15])
+    with cache.running(cache.next_token(step.sequences[:1])):
+        attn(x[:1])                                               # the eighth
+    step = cache.next_token(step.sequences[:1])
+    with cache.running(step), pytest.raises(ValueError, match="9 tokens"):
+        attn(x[:1])
+    # a step that is refilled, as a captured forward reads it
+    ids = cache.prompts([6, 5]).sequences
+    refilled = cache.reserve(2, 16)
+    with cache.running(refilled):
+        attn(x[:2])
+    for _ in range(2):
+        cache.next_token(ids, into=refilled)
+    free = cache.free_pages
+    with pytest.raises(ValueError, match="8 positions"):
+        cache.next_token(ids, into=refilled)
+    assert [cache.length(i) for i in ids] == [8, 7] and cache.free_pages == free and refilled.longest == 8
