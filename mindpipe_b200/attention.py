@@ -12,6 +12,7 @@ into a model.
 """
 from __future__ import annotations
 
+import threading
 from contextlib import contextmanager
 from dataclasses import dataclass
 
@@ -19,6 +20,8 @@ import torch
 from torch import nn
 
 from . import ops
+
+_entry = threading.Lock()        # of running(), for all caches: a cache can be copied with its model
 
 
 def rotary_table(inv_freq: torch.Tensor, max_positions: int, scaling: float = 1.0) -> torch.Tensor:
@@ -61,7 +64,8 @@ class PagedKVCache:
         step = cache.next_token(step.sequences)
 
     The bookkeeping is host code; running out of pages raises ``RuntimeError`` and changes nothing.  A step with a sequence
-    longer than the rotation's table raises ``ValueError`` in the forward, before anything is stored.
+    longer than the rotation's table raises ``ValueError`` in the forward, before anything is stored.  A cache is one thread's:
+    neither its bookkeeping nor its running step is shared (a second thread that runs a step meanwhile is refused).
     """
 
     def __init__(self, num_layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, *,
@@ -81,6 +85,7 @@ class PagedKVCache:
         self._length: dict[int, int] = {}
         self._next_id = 0
         self.step: Step | None = None
+        self._runner: int | None = None          # the thread whose step it is
 
     def layer(self, index: int) -> tuple[torch.Tensor, torch.Tensor]:
         """``k_cache, v_cache`` of a layer: ``[pages, kv_heads, page_size, head_dim]`` each."""
@@ -179,12 +184,17 @@ class PagedKVCache:
 
     @contextmanager
     def running(self, step: Step):
-        """The attached modules' forwards belong to ``step``."""
-        before, self.step = self.step, step
+        """The attached modules' forwards belong to ``step``.  One thread at a time: a second one raises ``RuntimeError``."""
+        me = threading.get_ident()
+        with _entry:
+            if self._runner not in (None, me):
+                raise RuntimeError("another thread is running a step of this cache")
+            before, self.step, self._runner = (self.step, self._runner), step, me
         try:
             yield step
         finally:
-            self.step = before
+            with _entry:
+                self.step, self._runner = before
 
 
 class PagedSelfAttention(nn.Module):

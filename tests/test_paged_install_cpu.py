@@ -279,3 +279,33 @@ def test_sequences_beyond_the_rotations_table_are_refused(monkeypatch):
     with pytest.raises(ValueError, match="8 positions"):
         cache.next_token(ids, into=refilled)
     assert [cache.length(i) for i in ids] == [8, 7] and cache.free_pages == free and refilled.longest == 8
+
+
+def test_a_second_thread_does_not_take_over_the_running_step():
+    import copy
+    import threading
+    cache, seen = make_cache(), []
+    one, two = cache.prompts([3]), cache.prompts([4])
+
+    def other():
+        try:
+            with cache.running(two):
+                seen.append("ran")
+        except RuntimeError as e:
+            seen.append(str(e))
+
+    def run():
+        thread = threading.Thread(target=other)
+        thread.start()
+        thread.join()
+
+    with cache.running(one):
+        run()
+        assert cache.step is one
+        with cache.running(two):                                  # within one thread steps nest
+            assert cache.step is two
+        assert cache.step is one
+        run()
+    run()
+    assert ["another thread" in s for s in seen] == [True, True, False] and cache.step is None
+    assert copy.deepcopy(cache).free_pages == cache.free_pages
