@@ -663,10 +663,10 @@ std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
   const uintptr_t first = reinterpret_cast<uintptr_t>(t.data_ptr());
   return {first, first + static_cast<uintptr_t>(last + 1) * t.element_size()};
 }
+using Span = std::pair<uintptr_t, uintptr_t>;
+bool apart(const Span& a, const Span& b) { return a.second <= b.first || b.second <= a.first; }
 bool apart(const at::Tensor& a, const at::Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0) return true;
-  const auto x = span_of(a), y = span_of(b);
-  return x.second <= y.first || y.second <= x.first;
+  return a.numel() == 0 || b.numel() == 0 || apart(span_of(a), span_of(b));
 }
 // Whether two 16-bit operands share memory, or a cache's entries with one another, where spans alone do not tell (the halves of
 // an interleaved pool): is there a sum of strides, each as often as the operands' sizes allow, that leads from one to the
@@ -717,8 +717,9 @@ struct Reach {
     return false;
   }
 };
+// (their spans meet)
 bool share(const at::Tensor& a, const at::Tensor& b) {
-  if (apart(a, b)) return false;
+  if (a.numel() == 0 || b.numel() == 0) return false;
   Reach r;
   r.add(a, true, false);
   r.add(b, false, true);
@@ -726,6 +727,10 @@ bool share(const at::Tensor& a, const at::Tensor& b) {
   return r.leads(0, (reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr())) / 16, true);
 }
 bool entries_share(const at::Tensor& t) {
+  const auto n = t.sizes(), stride = t.strides();
+  bool in_order = true;                      // each stride passes over all of what is inside it
+  for (size_t i = 0; i + 1 < n.size(); ++i) in_order = in_order && stride[i] >= n[i + 1] * stride[i + 1];
+  if (in_order) return false;
   Reach r;
   r.add(t, true, true);
   r.order();
@@ -766,9 +771,13 @@ PyObject* rotary_append(PyObject*, PyObject* args) {
   if (k->sizes() != v->sizes() || k->size(0) != t || k->size(2) != d || k->size(1) != cache.kv_heads || kc->size(3) != d)
     return call.fail("q, k, v and cache shapes are inconsistent"), nullptr;
   if (entries_share(*kc) || entries_share(*vc)) return call.fail("the cache's entries share memory (an expanded tensor)"), nullptr;
-  if (share(*kc, *vc)) return call.fail("k_cache and v_cache are the same memory, or overlap"), nullptr;
-  for (const at::Tensor* x : {q, k, v})
-    if (share(*x, *kc) || share(*x, *vc)) return call.fail("q, k or v overlaps the cache"), nullptr;
+  const Span kc_span = span_of(*kc), vc_span = span_of(*vc);
+  if (!apart(kc_span, vc_span) && share(*kc, *vc)) return call.fail("k_cache and v_cache are the same memory, or overlap"), nullptr;
+  for (const at::Tensor* x : {q, k, v}) {
+    const Span span = span_of(*x);
+    if ((!apart(span, kc_span) && share(*x, *kc)) || (!apart(span, vc_span) && share(*x, *vc)))
+      return call.fail("q, k or v overlaps the cache"), nullptr;
+  }
   if (q->size(1) == 0) return call.fail("q has no heads"), nullptr;
   if (pos->size(0) != t || slots->size(0) != t) return call.fail("positions and slots must have one entry per token"), nullptr;
   if (rotated < 2 || rotated % 2 || rotated > d || table->size(0) == 0 || reinterpret_cast<uintptr_t>(table->data_ptr()) % 16)
