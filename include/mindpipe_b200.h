@@ -755,6 +755,8 @@ int mp_gather_rows(const void* src, const void* row_map_i32, int n_dst_rows, int
  * are multiples of 16 bytes; strides count values and may not be negative; the last dimension is dense.
  * index_word (device int, may be null): set to 1 where a position, slot, page, length or sequence end that a kernel reads is
  * out of range.  Nothing outside the operands is touched then, and the results of the rows concerned are unspecified.
+ * Decode and prompts: scores, softmax and sums in fp32; the weights are rounded to dtype before the product with v, the result
+ * once more.
  */
 typedef struct {
   const void* data;            /* [rows, heads, D] */
@@ -788,9 +790,10 @@ int mp_rotary_append_paged(int dtype, const mp_head_rows* q, const mp_head_rows*
 /*
  * out[B,Hq,D] = softmax(scale q K^T) V over the first seq_lens[b] tokens in the pages page_table[b, :] names
  * (int32 [B, table_pages], entries behind the last token's page are not read); seq_lens[b] == 0 gives zeros.  Query head i
- * attends to the keys of head i / (Hq / kv_heads).  The cache is read once, split evenly over the SMs whatever the
- * lengths; parts of a sequence are joined through the workspace (zero-filled once when it is created, left so by every
- * call, not shared by calls that may overlap).  out may be q itself, if that is dense, and overlaps nothing else.
+ * attends to the keys of head i / (Hq / kv_heads).  The cache is read once for every 16 query heads of a head of keys, split
+ * evenly over the SMs whatever the lengths; parts of a sequence are joined through the workspace (zero-filled once when it is
+ * created, left so by every call, not shared by calls that may overlap).  out may be q itself, if that is dense, and overlaps
+ * nothing else.
  * Where ceil(B / 256) neighbouring sequences have some 2^29 tokens times kv_heads * ceil(Hq / kv_heads / 16) or more, the
  * lengths may count as out of range, and then no row of out is written.
  */

@@ -17,8 +17,8 @@
 // the tensor cores, the next scores have to be there when a group is done.  Tensor memory has 512 columns.  With heads of 128
 // values S and O take all of it, and a step goes through in two halves of 64 keys, each with its own place for S and P: while
 // one half is multiplied, the exponentials of the other are taken.  (2048 tokens of 32 heads: in whole steps 46.4 us, in
-// halves 41.5.  The products of 64 columns cost the tensor cores a quarter more time, which is why 8192 tokens of 64 heads, at
-// the power limit anyway, gained nothing: 1013, 1031.)  With heads of 64 values there is room for P beside S, and the next
+// halves 41.5.  The products of 64 columns cost the tensor cores a quarter more time, and 8192 tokens of 64 heads gained
+// nothing: 1013, 1031.)  With heads of 64 values there is room for P beside S, and the next
 // scores are sent for as soon as these are read (whole steps with P in S's place 540 us, halves 549, P apart 528).
 //
 // The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights stay in
@@ -45,8 +45,9 @@ constexpr int kWarps = 12, kThreads = 32 * kWarps;
 constexpr int kFewRegisters = 72, kManyRegisters = 216;
 constexpr int kTmemCols = 512;
 constexpr float kGrowth = 8.0f;                // log2 of how far a row's maximum may grow before it is taken
-// Weights are 2^(s - m + lift), rounded to the type before the product with V: below 2^15 in fp16, where many weights beneath
-// the type's 24 bits below 1 would be lost together.
+// Weights are 2^(s - m + lift), rounded to the type before the product with V, since that is what the tensor cores multiply (their
+// sum is of the unrounded ones; results are off by 2.6e-4 of their norm in fp16 and 2.0e-3 in bf16, with 32-bit weights 2.0e-4 and
+// 1.5e-3): below 2^15 in fp16, where many weights beneath the type's 24 bits below 1 would be lost together.
 template <typename T> constexpr float kLift = __is_same(T, __half) ? 15.0f - kGrowth : 0.0f;
 constexpr int kAhead = 4;                      // items that the planning warp is ahead
 constexpr int kSortedBatch = 256;              // sequences whose tiles are taken longest first
@@ -170,8 +171,9 @@ __device__ __forceinline__ float exp2_ordered(float x) {
 
 // Weights 2^(s scale - ref) of 16 scores, their sum added to `sum` and the weights rounded to eight words.  E of the eight
 // pairs are computed by multiplications while the exponential unit has the others: x = n + f with n the nearest integer, 2^f
-// by a polynomial of degree 5 (minimax on [-1/2, 1/2], found by exchange; relative error 2^-23.6), n added to the exponent.
-// x is at most about 2^7; below -127 it counts as -127, which gives 0.  (A NaN does not come through there: see the maximum.)
+// by a polynomial of degree 5 (minimax on [-1/2, 1/2], found by exchange; relative error 2^-22.6 with the constants rounded to
+// fp32, 2^-22.1 as evaluated), n added to the exponent.
+// x is at most about 2^7; below -127 it counts as -127, which gives 2^-149, 0 when rounded.  (A NaN does not come through there: see the maximum.)
 // The unit takes 16 values a clock and SM, 1024 clocks for a tile.  In this order, by hand, the instructions of a warp that
 // is alone on its scheduler keep it busy; as the compiler orders a plain loop they took 1650.  With none, one, two of eight by
 // multiplications: 2048 tokens of 32 heads 43.0, 42.5, 41.9 us, 8192 tokens of 64 heads 1085, 1070, 1050; prompts with heads
@@ -249,7 +251,8 @@ struct Work {
 // The items of a block, in turn, found by a warp.  With up to 256 sequences the tiles of rows are taken by how many keys they
 // have, longest first, and dealt to the blocks back and forth, so that all blocks have about as much to do (one prompt of
 // 2048 tokens and 32 heads dealt in one direction: a third of the SMs' time idle).  With more, in
-// the order of the batch.
+// the order of the batch.  (In order and by length: 40 prompts of about 200 tokens, of very different lengths, 100 and 80 us, 40
+// of 1000 1172 and 1175; 256 of 100 318 and 326, 256 of 400 1586 and 1510: with many tiles a block the order matters little.)
 struct Planner {
   const PrefillParams& p;
   int lane, rows, round = 0;

@@ -3,8 +3,8 @@
 //   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   s_j = scale q . k_j,   m = max_j s_j
 //
 // with a running m, sum and o, in one pass over the cache: 2 len Hkv D 16-bit values per sequence, which HBM bounds.  The
-// query heads that share a head of keys are the eight columns of the products S^T = K Q^T and O^T = V^T P^T, so keys and
-// values are read once for all of them (mma.sync: at HBM's rate an SM multiplies one 16 x 16 piece of the cache in about 10
+// query heads that share a head of keys are the columns, eight or sixteen, of the products S^T = K Q^T and O^T = V^T P^T, so
+// keys and values are read once for all of them (once for every sixteen, where there are more; mma.sync: at HBM's rate an SM multiplies one 16 x 16 piece of the cache in about 10
 // clocks, far below what even this path of the tensor cores takes; tcgen05's 128 rows would be 7/8 padding or more).
 //
 // All lengths are known on the device only (a captured launch serves every later step), so the work is cut there: the list of
@@ -31,11 +31,18 @@ using namespace attn;
 constexpr int kStages = 3;
 constexpr int kRows = 16;                                     // query heads per tile
 constexpr int kItemCost = 2;           // what an item costs beside its steps, in steps
-constexpr int kWholeSteps = 4;         // steps up to which an item is not cut: a join of teams takes 2-3 us
-// Weights are 2^(s - m + lift), rounded to the type before the product with V.  fp16 has no more than 24 bits below 1, and many
+// Steps up to which an item is not cut: a join of teams takes 2-3 us.  (Sequences of 300 tokens and eight heads, with 1, 4, 8:
+// 16 of them, 3 steps an item, 13.9, 8.4, 8.4 us; 19, 5 steps, 13.0, 13.0, 10.5; 64 21.9, 21.9, 19.1; 64 of 75 to 425
+// tokens 20.8, 21.0, 21.7; no difference from 2000 tokens on.)
+constexpr int kWholeSteps = 4;
+// Weights are 2^(s - m + lift), rounded to the type before the product with V, since that is what the tensor cores multiply
+// (results are off by 2.6e-4 of their norm in fp16 and 2.3e-3 in bf16, with 32-bit weights 2.1e-4 and 1.7e-3).  fp16 has no more than 24 bits below 1, and many
 // weights beneath those would be lost together; multiplied by 2^15 they keep all their bits down to 2^-29.
 template <typename T> constexpr float kLift = __is_same(T, __half) ? 15.0f : 0.0f;
-constexpr int kSoloTiles = 8;          // tiles of a sequence up to which a warp takes an item alone, if there are many items
+// Tiles of a sequence up to which a warp takes an item alone, if there are many items.  (301 sequences with five heads, of 60,
+// 130, 250 tokens on average, with 4, 8, 16 tiles: 15.2, 14.6, 14.6 us; 19.3, 21.5, 23.9; 27.8, 27.5, 33.4.  256 with eight
+// heads, of 100 tokens: 31.3, 30.1, 29.0.)
+constexpr int kSoloTiles = 8;
 
 // A team's two parts of items that it shares: the one it begins within (0) and the one it ends within (1).
 template <int DP>
@@ -604,8 +611,9 @@ int launch_decode(DecodeParams p, cudaStream_t st) {
 
 template <typename T, int DP, bool HALF, bool EIGHTS>
 int dispatch_teams(const DecodeParams& p, cudaStream_t st) {
-  // No more items than SMs: an SM's warps all go to one, which is then seldom cut (a sequence of 300 tokens and eight heads
-  // 8.7 us with teams of four warps).
+  // No more items than SMs: an SM's warps all go to one, which is then seldom cut.  (Eight heads; whole blocks, teams of four
+  // warps: 1 sequence of 300 tokens 7.5, 8.0 us, 16 of them 8.4, 11.3, 18 (144 items) 8.7, 12.8; 1 and 18 of 8000 16.4, 21.6
+  // and 97, 96.  Beyond: 24 of 2000 38.5, 38.7; 37 of 300 14.0, 12.4; 64 of 8000 329, 314.)
   return static_cast<long long>(p.batch) * p.items <= kSmCount ? launch_decode<T, DP, HALF, EIGHTS, true>(p, st)
                                                                : launch_decode<T, DP, HALF, EIGHTS, false>(p, st);
 }
@@ -615,6 +623,8 @@ int dispatch_rows(const DecodeParams& p, cudaStream_t st) {
 }
 template <typename T, int DP>
 int dispatch_pages(const DecodeParams& p, cudaStream_t st) {
+  // (16 tokens to a page and eight heads, pages looked up by eight rows, by the row: 64 sequences of 2000 tokens 87, 111 us;
+  // 1 of 300 7.5, 9.9)
   return p.by_page.d % 8 == 0 ? dispatch_rows<T, DP, true>(p, st) : dispatch_rows<T, DP, false>(p, st);
 }
 template <typename T>

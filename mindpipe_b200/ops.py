@@ -724,8 +724,8 @@ def rotary_append_paged(q, k, v, cos_sin, positions, slots, k_cache, v_cache, *,
     ``(2i, 2i + 1)``.  Token ``t`` goes to offset ``slots[t] % page_size`` of page ``slots[t] // page_size`` of
     ``k_cache`` / ``v_cache [pages, Hkv, page_size, D]`` (views with other strides included), or nowhere where
     ``slots[t] < 0`` (padding); a slot may occur once per call (of two tokens with the same one, parts of either may be
-    stored).  Views that share memory -- the two caches, a cache's entries, tokens within a cache -- raise ``ValueError``.  ``positions`` and ``slots`` are int32 ``[T]``.  Inference only, as the
-    attention operators: no gradients.
+    stored).  Views that share memory -- the two caches, a cache's entries, tokens within a cache -- raise ``ValueError``.
+    ``positions`` and ``slots`` are int32 ``[T]``.  Inference only, as the attention operators: no gradients.
 
     Returns ``(q_rotated, k_rotated | None)``; the caches are updated in place.  Positions and slots out of range touch no
     memory and raise at the next :func:`check_device_errors`.
@@ -743,9 +743,9 @@ def paged_attention_decode(q, k_cache, v_cache, page_table, seq_lens, *, scale: 
     ``q [B,Hq,D]`` fp16 or bf16, ``k_cache`` / ``v_cache [pages, Hkv, page_size, D]`` of the same type (``Hq`` a multiple of
     ``Hkv``), ``page_table`` int32 ``[B, pages of the longest]``, ``seq_lens`` int32 ``[B]``: tokens in the cache, the new
     one included; 0 gives a zero row.  What lies behind a sequence's end, in its last page and in its row of the table, is
-    never read.  ``scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``, where that is contiguous.  Nothing depends on
-    lengths known to the host: a captured call
-    serves whatever lengths the tensor holds at replay.  Pages and lengths out of range raise at the next
+    never read.  ``scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``, where that is contiguous.  Softmax and sums run in
+    fp32, the weights are rounded to the type before the product with the values.  Nothing depends on lengths known to the
+    host: a captured call serves whatever lengths the tensor holds at replay.  Pages and lengths out of range raise at the next
     :func:`check_device_errors`; so may lengths that add up to half a billion tokens times ``Hkv`` (times sixteens of queries
     to a head of keys) within ``ceil(B / 256)`` neighbouring sequences, and then no row of the result is written.
     """
@@ -760,7 +760,7 @@ def attention_prefill(q, k, v, cu_seqlens, *, scale: float | None = None, out=No
     """Causal attention within packed sequences: rows ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` are sequence ``b``.
 
     ``q [T,Hq,D]``, ``k`` and ``v [T,Hkv,D]`` fp16 or bf16, strided views included, ``Hq`` a multiple of ``Hkv``;
-    ``cu_seqlens`` int32 ``[B + 1]``, ascending, at most ``T``.  Returns ``out [T,Hq,D]``; rows that belong to no sequence
+    ``cu_seqlens`` int32 ``[B + 1]``, ascending, at most ``T``.  Arithmetic as in :func:`paged_attention_decode`.  Returns ``out [T,Hq,D]``; rows that belong to no sequence
     are left as they are in ``out``, and unspecified without one.  ``scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``,
     where that is contiguous.  Ends out of range or order leave all of ``out`` unspecified and raise at the next
     :func:`check_device_errors`.
