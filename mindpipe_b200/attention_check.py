@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import copy
 import inspect
+from contextlib import contextmanager
 
 import torch
 from torch import nn
@@ -33,6 +34,18 @@ class _Given(nn.Module):
     def forward(self, x, *args, **kwargs):
         self.seen.append(x)
         return self.values.view(*x.shape[:-1], -1)
+
+
+@contextmanager
+def _plain_torch():
+    """fp32 on the CPU, whatever the caller's defaults are."""
+    dtype = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    try:
+        with torch.no_grad(), torch.device("cpu"), torch.autocast("cpu", enabled=False):
+            yield
+    finally:
+        torch.set_default_dtype(dtype)
 
 
 def has_forward(module: nn.Module) -> bool:
@@ -85,13 +98,12 @@ def _clone(attention: nn.Module, projections: dict[str, nn.Module]) -> nn.Module
             clone._modules[name] = copy.deepcopy(child).cpu().eval()
     config = getattr(attention, "config", None)
     if config is not None:
-        clone.config = copy.copy(config)
+        clone.config = copy.deepcopy(config)                      # (setting it reaches the configs inside)
         if hasattr(config, "_attn_implementation"):
             clone.config._attn_implementation = "eager"
     return clone
 
 
-@torch.no_grad()
 def check_attention(attention: nn.Module, name: str, *, head_dim: int, rotated: int, scale: float | None) -> None:
     """``attention`` computes ``o_proj(softmax(scale rot(q) rot(k)^T, causal) v)`` of its own projections, heads in groups."""
     dropped = [n for n, p in attention._parameters.items() if p is not None] + \
@@ -100,7 +112,11 @@ def check_attention(attention: nn.Module, name: str, *, head_dim: int, rotated: 
         raise ValueError(f"{name}: {', '.join(dropped)} is not part of the paged attention")
     if not has_forward(attention):
         return                                                    # projections and nothing else: there is no code to differ
-    scale = head_dim ** -0.5 if scale is None else float(scale)
+    with _plain_torch():
+        _compare(attention, name, head_dim, rotated, head_dim ** -0.5 if scale is None else float(scale))
+
+
+def _compare(attention, name, head_dim, rotated, scale):
     g = torch.Generator().manual_seed(0)
     # scores of a few units, so that caps and norms show; large values, so that clamps do
     size = (4.0 / max(abs(scale) * head_dim ** 0.5, 1e-6)) ** 0.5
@@ -129,17 +145,17 @@ def check_attention(attention: nn.Module, name: str, *, head_dim: int, rotated: 
                          "(projections, rotation in halves, causal softmax, nothing else)")
 
 
-@torch.no_grad()
 def check_table(rotary: nn.Module, cos_sin: torch.Tensor) -> None:
     """``cos_sin`` holds what ``rotary(x, position_ids)`` returns: cosines and sines, each twice in halves."""
     if not has_forward(rotary):
         return
     rows, half = cos_sin.shape[0], cos_sin.shape[1] // 2
-    ids = torch.tensor(sorted({0, 1, 2, 3, rows // 2, rows - 1} & set(range(rows))))
+    ids = torch.tensor(sorted(p for p in {0, 1, 2, 3, rows // 2, rows - 1} if p < rows), device="cpu")
     table = cos_sin[ids.to(cos_sin.device)].cpu()
     want = [torch.cat([x, x], -1)[None] for x in (table[:, :half], table[:, half:])]
     try:
-        got = type(rotary).forward(copy.deepcopy(rotary).cpu(), torch.zeros(1, len(ids), 1), ids[None])
+        with _plain_torch():
+            got = type(rotary).forward(copy.deepcopy(rotary).cpu(), torch.zeros(1, len(ids), 1), ids[None])
         # (the model's angles are taken in 32 bits)
         same = len(got) == 2 and all(g.shape == w.shape and bool(((g.double() - w).abs() <= 1e-4 + ids[None, :, None] * 2.0 ** -22).all())
                                      for g, w in zip(got, want))
@@ -163,7 +179,7 @@ def check_config(config, name: str, layer: int, positions: int) -> None:
         if kind is not None and not windows:
             raise ValueError(f"{name}: {kind} without its size in the config")
         for key, size in windows.items():
-            if size < positions:
+            if not isinstance(size, int) or size < positions:
                 raise ValueError(f"{name}: {key} of {size} is less than the table's {positions} positions, and not part of the paged "
                                  "attention (max_positions up to it is)")
     if get("use_bidirectional_attention", False) or get("is_causal", True) is False:

@@ -188,6 +188,9 @@ def install_paged_attention(model: nn.Module, cache: PagedKVCache, *, cos_sin: t
         raise ValueError(f"the model has {len(layers)} layers, the cache {cache.pool.shape[0]}")
     if cos_sin is None:
         cos_sin = _model_table(model, backbone, max_positions, cache.pool.device)
+    if cos_sin.dim() != 2 or cos_sin.shape[0] < 1 or cos_sin.shape[1] % 2 or not 2 <= cos_sin.shape[1] <= cache.pool.shape[-1]:
+        raise ValueError(f"cos_sin must be [positions, rotated] with an even number of rotated values up to the cache's heads of "
+                         f"{cache.pool.shape[-1]}, got {tuple(cos_sin.shape)}")
     made = []
     for i, layer in enumerate(layers):
         attn, name = getattr(layer, "self_attn", None), f"{prefix}.{i}.self_attn"

@@ -309,3 +309,37 @@ def test_a_second_thread_does_not_take_over_the_running_step():
     run()
     assert ["another thread" in s for s in seen] == [True, True, False] and cache.step is None
     assert copy.deepcopy(cache).free_pages == cache.free_pages
+
+
+@pytest.mark.parametrize("default", [torch.float16, torch.float64, "meta"])
+def test_the_callers_defaults_do_not_enter(default):
+    model = build("llama")
+    before = torch.get_default_dtype()
+    try:
+        if default == "meta":
+            with torch.device("meta"):
+                cache = make_cache(4, 2, 32)
+                install.install_paged_attention(model, cache, cos_sin=rotary_table(torch.ones(16, device="cpu"), 128))
+        else:
+            torch.set_default_dtype(default)
+            install.install_paged_attention(model, make_cache(4, 2, 32))
+            assert torch.get_default_dtype() == default
+    finally:
+        torch.set_default_dtype(before)
+    assert isinstance(model.model.layers[3].self_attn, PagedSelfAttention)
+    assert model.config._attn_implementation == "eager"
+
+
+def test_the_models_config_is_left_alone():
+    transformers = pytest.importorskip("transformers")
+    config = transformers.AutoConfig.for_model("llama", **SMALL)
+    model = transformers.AutoModelForCausalLM.from_config(config, attn_implementation="sdpa").eval()
+    install.install_paged_attention(model, make_cache(4, 2, 32))
+    assert model.config._attn_implementation == "sdpa"
+
+
+def test_a_table_that_does_not_fit_the_heads_is_refused():
+    for bad in (torch.ones(8, 66), torch.ones(8, 63), torch.ones(8, 0), torch.ones(0, 64), torch.ones(64)):
+        model = build("llama", head_dim=64)
+        with pytest.raises(ValueError, match="cos_sin must be"):
+            install.install_paged_attention(model, make_cache(4, 2, 64), cos_sin=bad)
