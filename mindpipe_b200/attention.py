@@ -128,8 +128,8 @@ class PagedKVCache:
     def next_token(self, sequences, into: Step | None = None) -> Step:
         """One token more for each of the sequences.
 
-        ``into``: an earlier step of as many sequences, whose tensors are written instead of new ones -- a captured forward
-        then runs the new step when replayed.  Its table keeps its width: sequences that outgrow it raise ``ValueError``
+        ``into``: an earlier step of as many sequences, whose tensors are written instead of new ones, on the current stream -- a
+        captured forward then runs the new step when replayed there.  Its table keeps its width: sequences that outgrow it raise ``ValueError``
         (:meth:`reserve` makes a wider one), and so do sequences that outgrow the rotation's table of the forward."""
         sequences = list(sequences)
         if len(set(sequences)) != len(sequences):
