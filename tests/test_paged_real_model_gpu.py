@@ -45,3 +45,24 @@ def test_prompts_then_tokens_of_real_models(kind, settings, dtype):
         want = plain(s[None], use_cache=False).logits[0].double()
         assert ((torch.cat(mine).double() - want).norm() / want.norm()).item() <= TOL[dtype]
     ops.check_device_errors()
+
+
+@pytest.mark.parametrize("linears", ["w4a16", "w8a8"])
+@torch.no_grad()
+def test_real_models_with_quantised_linears_are_asked_too(linears):
+    """The installers of the linears first: the attention's code is the same, whatever its projections are."""
+    model = build("llama", hidden_size=256, head_dim=64, intermediate_size=512).to("cuda", torch.float16)
+    if linears == "w4a16":
+        install.real_quantize_model_weight(model, 4, {"zero_point": True, "q_group_size": 128})
+    else:
+        install.quantize_model(model, weight_bits=8, activation_bits=8, act_quant="per_token")
+    ids = torch.randint(3, 128, (40,), generator=torch.Generator().manual_seed(3)).cuda()
+    want = model(ids[None], use_cache=False).logits[0].double()
+    cache = PagedKVCache(4, 10, 8, 2, 64)
+    install.install_paged_attention(model, cache)
+    step = cache.prompts([40])
+    with cache.running(step):
+        got = model(ids[None], position_ids=step.positions.long()[None], use_cache=False).logits[0].double()
+    # the same linears on inputs that differ by roundings; W8A8 rounds rows to 8 bits, and a step of a code is 2^-7 of the largest
+    assert ((got - want).norm() / want.norm()).item() <= {"w4a16": 1e-2, "w8a8": 5e-2}[linears]
+    ops.check_device_errors()
